@@ -5,7 +5,8 @@ for the layers that keep that.
 Layers with the same need form a group with storage of its own:
   * a KV group: pool[layer, page, 2 (K, V), kv head, row, head_dim] in the
     model's dtype (one flat row a page where keys and values differ in size or
-    the values lie inside the keys' rows), pages of ``page_size`` tokens handed
+    the values lie inside the keys' rows; pool[layer, page, kv head, bytes] where
+    rows are held in 4 bits), pages of ``page_size`` tokens handed
     out on demand; a group with a window gives pages back as they fall out of it;
   * a state group: state[layer, slot, ...] in the need's dtype (float32 unless it
     says otherwise), zeroed when the slot is assigned.
@@ -92,7 +93,8 @@ def plan_cache(needs: Sequence[Union[Need, Sequence[Need]]], cache_of: Sequence[
 class KVView:
     """What an attention-like mixer gets: its layer's pool, and the page table
     of the step's sequences (device int32 [B, P])."""
-    pool: torch.Tensor                 # [pages, 2, kv heads, page_size, head_dim]; [pages, page elements] if need.uneven
+    pool: torch.Tensor                 # [pages, 2, kv heads, page_size, head_dim]; [pages, page elements] if need.uneven;
+    #                                    uint8 [pages, kv heads, page_size * (head_dim + 8)] if need.bits
     page_table: torch.Tensor
     page_size: int
     writable: bool
@@ -106,6 +108,16 @@ class StateView:
     state: torch.Tensor
     writable: bool
     need: StateNeed
+
+
+def rows_of_4_bits(pages: torch.Tensor, page_size: int, head_dim: int) -> torch.Tensor:
+    """What pages held in 4 bits stand for: uint8 [..., kv heads, page_size * (head_dim + 8)] -> float32
+    [..., 2, kv heads, page_size, head_dim].  For inspection, on any device; steps read rows back with kernels."""
+    codes = pages[..., :page_size * head_dim].unflatten(-1, (2, page_size, head_dim // 2))
+    codes = torch.stack([codes & 15, codes >> 4], dim=-1).flatten(-2).float()
+    params = pages[..., page_size * head_dim:].contiguous().view(torch.bfloat16).unflatten(-1, (page_size, 2, 2)).float()
+    params = params.transpose(-3, -2)                      # [..., kv heads, K or V, row, (step, zero)]
+    return (params[..., 1:2] + codes * params[..., 0:1]).movedim(-3, -4)
 
 
 class _Slot:
@@ -143,11 +155,13 @@ class SequenceCache:
         self._state_views: Dict[int, List[List[torch.Tensor]]] = {}     # slot -> its state in every layer, a list a dtype
         for gi, g in enumerate(plan.groups):
             if isinstance(g.need, KVNeed):
-                if g.need.uneven:
+                if g.need.bits:
+                    shape = (g.n_layers, max(n_pages, 1), g.need.n_kv_heads, page_size * (g.need.head_dim + 8))
+                elif g.need.uneven:
                     shape = (g.n_layers, max(n_pages, 1), g.need.page_elements(page_size))
                 else:
                     shape = (g.n_layers, max(n_pages, 1), 2, g.need.n_kv_heads, page_size, g.need.head_dim)
-                self.storage[gi] = torch.zeros(shape, dtype=dtype, device=self.device)
+                self.storage[gi] = torch.zeros(shape, dtype=torch.uint8 if g.need.bits else dtype, device=self.device)
             else:
                 shape = (g.n_layers, max(n_slots, 1)) + tuple(g.need.shape)
                 self.storage[gi] = torch.zeros(shape, dtype=g.need.dtype, device=self.device)
@@ -335,7 +349,7 @@ class SequenceCache:
     # ---- inspection ---------------------------------------------------------------
     def dump_slot(self, slot: int) -> Dict[int, torch.Tensor]:
         """Contents of a sequence for tests: per KV group [layers, 2, length, kv heads, head_dim]
-        (rows of pages that were given back are zero; a group whose values differ in size from its keys
+        (rows of pages that were given back are zero; float32 for a group held in 4 bits; a group whose values differ in size from its keys
         gives a pair (keys [layers, length, kv heads, head_dim], values [layers, length, kv heads, v_dim])),
         per state group [layers, ...]."""
         seq = self._get(slot)
@@ -358,13 +372,14 @@ class SequenceCache:
                 out[gi] = (ks, vs)
             elif isinstance(g.need, KVNeed):
                 L = int(self._len[slot])
-                rows = torch.zeros((g.n_layers, 2, L, g.need.n_kv_heads, g.need.head_dim), dtype=st.dtype,
-                                   device=st.device)
+                rows = torch.zeros((g.n_layers, 2, L, g.need.n_kv_heads, g.need.head_dim),
+                                   dtype=torch.float32 if g.need.bits else st.dtype, device=st.device)
                 for blk, page in enumerate(seq.pages[gi]):
                     lo, hi = blk * self.page_size, min(L, (blk + 1) * self.page_size)
                     if page is None or lo >= hi:
                         continue
-                    rows[:, :, lo:hi] = st[:, page, :, :, :hi - lo].permute(0, 1, 3, 2, 4)
+                    held = rows_of_4_bits(st[:, page], self.page_size, g.need.head_dim) if g.need.bits else st[:, page]
+                    rows[:, :, lo:hi] = held[:, :, :, :hi - lo].permute(0, 1, 3, 2, 4)
                 out[gi] = rows
             else:
                 out[gi] = st[:, slot].clone()

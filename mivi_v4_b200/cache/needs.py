@@ -20,7 +20,9 @@ class KVNeed:
     keys of its own chunk of ``chunk`` positions, counted from the sequence's start, so the pages that lie wholly
     before the chunk of the next token are given back.  ``values_in_keys``: the values are the first ``v_dim``
     elements of the keys' rows (a compressed cache that all heads read), so a page holds rows only:
-    [kv head][row][head_dim]."""
+    [kv head][row][head_dim].  ``bits`` 4: rows are held as 4-bit codes with a step and a zero each
+    (``ops.kernels.kv4_prepare``), a page being ``n_kv_heads`` runs of ``page_size * (head_dim + 8)`` bytes; 0: in the
+    model's dtype."""
     n_kv_heads: int
     head_dim: int
     window: int = 0
@@ -28,6 +30,7 @@ class KVNeed:
     keep_first: int = 0
     chunk: int = 0
     values_in_keys: bool = False
+    bits: int = 0
 
     @property
     def value_dim(self) -> int:

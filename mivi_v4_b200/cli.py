@@ -35,6 +35,9 @@ def _ids(text: str) -> List[int]:
         raise argparse.ArgumentTypeError(f"not a list of token ids: {text!r}") from None
 
 
+CACHE_HELP = "int4: keys and values are held in 4 bits (grouped-query attention only); default: in the model's dtype"
+
+
 def build_parser() -> argparse.ArgumentParser:
     ap = argparse.ArgumentParser(prog="mivi_v4_b200", description="LFM2 / LFM2.5 generation on one B200")
     sub = ap.add_subparsers(dest="command", required=True)
@@ -56,6 +59,7 @@ def build_parser() -> argparse.ArgumentParser:
     g.add_argument("-c", "--ctx-size", type=int, default=None, help="most tokens of one sequence (default: from the model, else 16384)")
     g.add_argument("--stop-ids", type=_ids, default=None, help="token ids that end a sequence (default: the model's eos)")
     g.add_argument("--dtype", default="bfloat16", choices=["bfloat16", "float32"])
+    g.add_argument("--cache-dtype", default=None, choices=["int4"], help=CACHE_HELP)
     g.add_argument("--max-batch", type=int, default=64, help="most sequences that run together")
     g.add_argument("--json", action="store_true", help="print one JSON object instead of lines of ids")
 
@@ -77,6 +81,7 @@ def build_parser() -> argparse.ArgumentParser:
     rp.add_argument("--dtype", required=True, choices=["bfloat16", "float32"])
     rp.add_argument("--out", required=True)
     rp.add_argument("--max-tokens", type=int, required=True)
+    rp.add_argument("--cache-dtype", default=None, choices=["int4"], help=CACHE_HELP)
 
     b = sub.add_parser("bench", help="prefill and decode throughput of a model folder")
     b.add_argument("-m", "--model", default=None, help="model folder")
@@ -87,6 +92,7 @@ def build_parser() -> argparse.ArgumentParser:
     b.add_argument("--steps", type=int, default=64, help="timed decode steps")
     b.add_argument("--profile", action="store_true", help="also print where a step's time goes, by stage and kernel")
     b.add_argument("--dtype", default="bfloat16", choices=["bfloat16", "float32"])
+    b.add_argument("--cache-dtype", default=None, choices=["int4"], help=CACHE_HELP)
     return ap
 
 
@@ -104,7 +110,7 @@ def cmd_generate(a) -> int:
     model.spec.max_positions = ctx
     longest = max(len(p) for p in prompts) + a.max_tokens
     batch = min(a.max_batch, len(prompts))
-    eng = Engine(model, max_tokens=batch * (min(ctx, longest) + 64), max_batch=batch)
+    eng = Engine(model, max_tokens=batch * (min(ctx, longest) + 64), max_batch=batch, cache_dtype=a.cache_dtype)
     sp = SamplingParams(temperature=a.temp, top_p=a.top_p, top_k=a.top_k, min_p=a.min_p,
                         repetition_penalty=a.rep_penalty, presence_penalty=a.presence_penalty,
                         frequency_penalty=a.frequency_penalty, seed=a.seed)
@@ -190,10 +196,11 @@ def cmd_bench(a) -> int:
         print("bench: give a model folder (-m) or a config.json for random weights (--config)", file=sys.stderr)
         return 2
     T, B = a.bench_prompt_tokens, a.batch
-    nums = measure.model_numbers(model)
-    pre_ms = measure.prefill_run(model, T, reps=3, warmup=2)
-    dec = measure.decode_run(model, [a.prompt_tokens] * B, a.steps, warmup=4)
-    gen = measure.generate_run(model, [a.prompt_tokens] * B, a.steps + 1)
+    cd = a.cache_dtype
+    nums = measure.model_numbers(model, cd)
+    pre_ms = measure.prefill_run(model, T, reps=3, warmup=2, cache_dtype=cd)
+    dec = measure.decode_run(model, [a.prompt_tokens] * B, a.steps, warmup=4, cache_dtype=cd)
+    gen = measure.generate_run(model, [a.prompt_tokens] * B, a.steps + 1, cache_dtype=cd)
     step_bytes = nums["weight_bytes"] + B * (dec["cached_tokens_mean"] * nums["kv_bytes_per_token"]
                                              + nums["state_bytes_per_seq"])
     pre_flops = T * nums["gemm_flops_per_token"] + nums["head_flops_per_row"] + nums["attn_flops"](T)
@@ -204,15 +211,16 @@ def cmd_bench(a) -> int:
         "decode_gb_per_s": step_bytes / (dec["ms_per_step"] * 1e-3) / 1e9,
         "generate_tok_s": gen["decode_tokens_per_s"], "kernels_per_step": dec["launches"] / a.steps}))
     if a.profile:
-        measure.print_stage_report(measure.stage_report(model, [a.prompt_tokens] * B),
+        measure.print_stage_report(measure.stage_report(model, [a.prompt_tokens] * B, cache_dtype=cd),
                                    f"decode step, {B} sequence(s) of {a.prompt_tokens} cached tokens")
-        measure.print_stage_report(measure.stage_report(model, [T], prefill=True), f"prefill of {T} tokens")
+        measure.print_stage_report(measure.stage_report(model, [T], prefill=True, cache_dtype=cd), f"prefill of {T} tokens")
     return 0
 
 
 def cmd_replay(a) -> int:
     from .replay import main as replay_main
-    return replay_main(["--model", a.model, "--dtype", a.dtype, "--out", a.out, "--max-tokens", str(a.max_tokens)])
+    return replay_main(["--model", a.model, "--dtype", a.dtype, "--out", a.out, "--max-tokens", str(a.max_tokens)]
+                       + (["--cache-dtype", a.cache_dtype] if a.cache_dtype else []))
 
 
 def main(argv=None) -> int:

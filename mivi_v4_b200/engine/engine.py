@@ -52,7 +52,7 @@ def _width_for(blocks: int) -> int:
 class Engine:
     def __init__(self, model: Model, *, max_tokens: int, max_batch: Optional[int] = None,
                  page_size: int = 64, max_step_tokens: int = 8192, cuda_graphs: bool = True,
-                 max_graphs: int = 64, profile: bool = False):
+                 max_graphs: int = 64, profile: bool = False, cache_dtype: Optional[str] = None):
         if model.dtype is None:
             raise ValueError("the model has no weights yet; use load_model()")
         if model.device.type != "cuda":
@@ -65,7 +65,9 @@ class Engine:
         # every live sequence holds at least one page, so there are never more sequences than pages
         n_slots = max_batch if max_batch is not None else min(n_pages, 256)
         self.max_batch = max(1, n_slots)
-        self.plan = model.cache_plan()
+        # "int4": keys and values are held as 4-bit codes with a step and a zero a row (36 bytes a row of 64 against 128)
+        self.cache_dtype = cache_dtype
+        self.plan = model.cache_plan(cache_dtype)
         self.cache = SequenceCache(self.plan, n_slots=self.max_batch, n_pages=n_pages, page_size=page_size,
                                    dtype=self.dtype, device=self.device)
         self.ws = Workspace(self.device)

@@ -4,16 +4,20 @@ architecture; the architecture's file supplies the ``ModelSpec``.
 """
 from __future__ import annotations
 
+from dataclasses import replace
 from typing import Dict, List, Optional
 
 import torch
 
 from .. import architectures  # noqa: F401  (registers the architectures that ship with the package)
-from ..cache import CachePlan, plan_cache
+from ..cache import CacheError, CachePlan, KVNeed, plan_cache
 from ..config import architecture_for
 from ..ops import kernels as K
 from ..ops.linear import end_norms_carried
 from ..parts import ModelSpec, ParamSpec, build
+
+
+CACHE_DTYPES = (None, "int4")
 
 
 class _AfterLastBlock:
@@ -93,15 +97,29 @@ class Model:
         return sum(self.weight_extents().values())
 
     # ---- cache --------------------------------------------------------------
-    def cache_plan(self) -> CachePlan:
+    def cache_plan(self, cache_dtype: Optional[str] = None) -> CachePlan:
         """One position per schedule entry; an embedding that keeps something per sequence (the previous token)
-        has the position after the last entry."""
+        has the position after the last entry.  ``cache_dtype`` "int4": keys and values are held in 4 bits (states as ever)."""
+        if cache_dtype not in CACHE_DTYPES:
+            raise ValueError(f"cache_dtype {cache_dtype!r}; known: None (the model's dtype), \"int4\"")
         needs = [self.blocks[e.block].cache_need() for e in self.schedule]
+        if cache_dtype == "int4":
+            needs = [self._in_4_bits(self.blocks[e.block], n) for e, n in zip(self.schedule, needs)]
         cache_of = [e.cache_of for e in self.schedule]
         if self.embedding.cache_need() is not None:
             needs.append(self.embedding.cache_need())
             cache_of.append(None)
         return plan_cache(needs, cache_of)
+
+    @staticmethod
+    def _in_4_bits(block, need):
+        if not any(isinstance(n, KVNeed) for n in (need if isinstance(need, (list, tuple)) else [need])):
+            return need
+        mixer = getattr(block, "mixer", None)
+        if not getattr(mixer, "holds_4_bits", False) or not isinstance(need, KVNeed):
+            raise CacheError(f"cache_dtype \"int4\": the mixer {getattr(mixer, 'kind', type(block).__name__)!r} keeps its keys and "
+                             "values in the model's dtype only")
+        return replace(need, bits=4)
 
     # ---- one step ---------------------------------------------------------------
     def forward(self, step, cache) -> Optional[torch.Tensor]:

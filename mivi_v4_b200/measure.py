@@ -20,14 +20,14 @@ from .cache import KVNeed
 from .ops import kernels as K
 
 
-def model_numbers(model) -> dict:
+def model_numbers(model, cache_dtype: Optional[str] = None) -> dict:
     """Bytes and floating-point operations of the model's steps, from the model itself: the bytes
     of all its tensors (a decode step reads each once), the cache bytes a token and a sequence
     hold, the matrix-product operations a token costs in the layers and a row of logits in the
     head, and the attention operations of a prompt of T tokens."""
     elt = 2 if model.dtype == torch.bfloat16 else 4
-    plan = model.cache_plan()
-    kv_per_token = sum(g.n_layers * g.need.n_kv_heads * (g.need.head_dim + g.need.value_dim) * elt
+    plan = model.cache_plan(cache_dtype)
+    kv_per_token = sum(g.n_layers * g.need.n_kv_heads * (g.need.head_dim + 8 if g.need.bits else (g.need.head_dim + g.need.value_dim) * elt)
                        for g in plan.groups if isinstance(g.need, KVNeed))
     state_per_seq = sum(g.n_layers * torch.empty(0, dtype=g.need.dtype).element_size() * math.prod(g.need.shape)
                         for g in plan.groups if not isinstance(g.need, KVNeed))
@@ -86,7 +86,7 @@ def _engine(model, prompt_lens, new_tokens, **kw):
 
 
 def decode_run(model, prompt_lens: Sequence[int], steps: int, warmup: int, seed: int = 0,
-               room_each: Optional[int] = None) -> dict:
+               room_each: Optional[int] = None, cache_dtype: Optional[str] = None) -> dict:
     """Device time of exactly ``steps`` decode steps of sequences that hold prompts of ``prompt_lens``
     tokens, greedy sampling on the device included, host token ids in.  Also times the unequal prefill
     step that fills the cache.  ``room_each``: cache room per sequence (default: what the run needs)."""
@@ -95,9 +95,9 @@ def decode_run(model, prompt_lens: Sequence[int], steps: int, warmup: int, seed:
     V = model.vocab_size
     total = warmup + steps
     if room_each is not None:
-        eng = Engine(model, max_tokens=B * room_each, max_batch=B)
+        eng = Engine(model, max_tokens=B * room_each, max_batch=B, cache_dtype=cache_dtype)
     else:
-        eng = _engine(model, prompt_lens, total + 1)
+        eng = _engine(model, prompt_lens, total + 1, cache_dtype=cache_dtype)
     prompts = random_prompts(V, prompt_lens, seed)
     g = torch.Generator().manual_seed(seed + 1)
     feed = torch.randint(0, V, (total, B), generator=g).tolist()
@@ -141,10 +141,10 @@ def decode_run(model, prompt_lens: Sequence[int], steps: int, warmup: int, seed:
     return res
 
 
-def prefill_run(model, tokens: int, reps: int, warmup: int, seed: int = 2) -> float:
+def prefill_run(model, tokens: int, reps: int, warmup: int, seed: int = 2, cache_dtype: Optional[str] = None) -> float:
     """Median device time (ms) of one prompt of ``tokens`` tokens in one step, last logits wanted."""
     from .engine import Engine
-    eng = Engine(model, max_tokens=2 * tokens + 128, max_batch=2, max_step_tokens=tokens)
+    eng = Engine(model, max_tokens=2 * tokens + 128, max_batch=2, max_step_tokens=tokens, cache_dtype=cache_dtype)
     g = torch.Generator().manual_seed(seed)
     times = []
     for i in range(warmup + reps):
@@ -165,13 +165,14 @@ def prefill_run(model, tokens: int, reps: int, warmup: int, seed: int = 2) -> fl
     return statistics.median(times)
 
 
-def generate_run(model, prompt_lens: Sequence[int], new_tokens: int, warmup_tokens: int = 4, seed: int = 1) -> dict:
+def generate_run(model, prompt_lens: Sequence[int], new_tokens: int, warmup_tokens: int = 4, seed: int = 1,
+                 cache_dtype: Optional[str] = None) -> dict:
     """Through the public entry point: host token lists in, host token lists out, one host-to-device copy
     of the step's inputs and one device-to-host read of the sampled tokens every step.  Decoding is timed
     by the host's clock from the first emitted token to the return, as the reference times generation
     without its first token; the prefill from the call to the first token."""
     from .sampling import SamplingParams
-    eng = _engine(model, prompt_lens, max(new_tokens, warmup_tokens) + 1)
+    eng = _engine(model, prompt_lens, max(new_tokens, warmup_tokens) + 1, cache_dtype=cache_dtype)
     prompts = random_prompts(model.vocab_size, prompt_lens, seed)
     # the same lengths as the timed run: its decode steps then find their shapes recorded
     eng.generate(prompts, warmup_tokens, SamplingParams.greedy(), stop_token_ids=[])
@@ -201,13 +202,15 @@ def generate_run(model, prompt_lens: Sequence[int], new_tokens: int, warmup_toke
     return res
 
 
-def stage_report(model, prompt_lens: Sequence[int], steps: int = 8, prefill: bool = False, seed: int = 3) -> dict:
+def stage_report(model, prompt_lens: Sequence[int], steps: int = 8, prefill: bool = False, seed: int = 3,
+                 cache_dtype: Optional[str] = None) -> dict:
     """Where the time of decode steps (or of the prefill step) goes: an engine with ``profile=True`` runs
     them launch by launch with every launch timed; see ``KernelProfile.report``."""
     from .engine import Engine
     B = len(prompt_lens)
     room = sum(-(-(n + steps + 8) // 64) * 64 for n in prompt_lens)
-    eng = Engine(model, max_tokens=room, max_batch=B, profile=True, max_step_tokens=max(8192, max(prompt_lens)))
+    eng = Engine(model, max_tokens=room, max_batch=B, profile=True, max_step_tokens=max(8192, max(prompt_lens)),
+                 cache_dtype=cache_dtype)
     prompts = random_prompts(model.vocab_size, prompt_lens, seed)
     slots = [eng.open() for _ in range(B)]
     eng.step(list(zip(slots, prompts)), "last", copy=False)           # compiles nothing new later

@@ -48,6 +48,10 @@ _SIGNATURES = {
         "mv_attention_generic": [_P, _P, _Q, _P, _I, _I, _P, _P, _P, _I, _I, _I, _I, _I, _F, _I, _I, _P],
         "mv_attention_decode": [_P, _P, _Q, _P, _I, _I, _P, _P, _P, _I, _P, _P, _P, _I, _I, _I, _I, _F, _I, _I,
                                 _I, _I, _P],
+        "mv_kv4_prepare": [_P, _P, _P, _F, _P, _I, _P, _P, _P, _I, _I, _P, _P, _I, _I, _I, _I, _I, _P],
+        "mv_kv4_read": [_P, _P, _I, _I, _P, _P, _P, _P, _I, _I, _I, _I, _P],
+        "mv_kv4_read_pages": [_P, _P, _I, _I, _P, _P, _I, _P, _I, _P, _I, _I, _I, _I, _P],
+        "mv_attention_kv4": [_P, _P, _P, _I, _I, _P, _P, _P, _I, _P, _P, _P, _I, _I, _I, _I, _F, _I, _I, _I, _I, _P],
         "mv_layernorm": [_P, _P, _P, _P, _I, _P, _I, _I, _F, _P],
         "mv_gated_rmsnorm": [_P, _P, _I, _P, _I, _P, _I, _I, _I, _I, _F, _I, _P],
         "mv_rmsnorm_add": [_P, _P, _P, _I, _I, _F, _P],
@@ -2614,6 +2618,215 @@ def attention_prefill_tc(q: torch.Tensor, pool: torch.Tensor, page_table, cu, st
         _need(out, "attention out", None, (N, nh * hd)), N, n_seqs, nh, nkv, float(scale),
         _error_flag(q.device).data_ptr(), _stream()), "mv_attention_prefill_tc")
     return out
+
+
+# ---- a cache held in 4 bits --------------------------------------------------------------------------------------
+def kv4_page_bytes(page_size: int, hd: int) -> int:
+    """Bytes of one kv head in a page held in 4 bits: codes of keys and values, and a step and a zero for every row of each."""
+    return page_size * (hd + 8)
+
+
+def _check_kv4(pool: torch.Tensor, nkv: int, hd: int, what: str) -> int:
+    """The page size of a 4-bit pool, uint8 [pages, kv heads, page_size * (head size + 8)]."""
+    if hd % 8 or not 8 <= hd <= MAX_HEAD_DIM:
+        raise KernelError(f"{what}: head size {hd} must be a multiple of 8 and at most {MAX_HEAD_DIM}")
+    if nkv < 1:
+        raise KernelError(f"{what}: {nkv} kv heads")
+    if pool.dtype != torch.uint8 or pool.dim() != 3 or pool.shape[1] != nkv or pool.shape[2] < 1 or pool.shape[2] % (hd + 8):
+        raise KernelError(f"{what}: a cache in 4 bits is uint8 [pages, {nkv}, page size * {hd + 8}], got {pool.dtype} {tuple(pool.shape)}")
+    page_size = pool.shape[2] // (hd + 8)
+    if page_size & (page_size - 1):
+        raise KernelError(f"{what}: page size {page_size} is not a power of two")
+    if pool.data_ptr() % 16:
+        raise KernelError(f"{what}: the cache pool must start on 16 bytes")
+    return page_size
+
+
+def _check_table(page_table: torch.Tensor, what: str) -> int:
+    _need(page_table, "page table", torch.int32)
+    if page_table.dim() != 2 or page_table.shape[1] < 1:
+        raise KernelError(f"{what}: page table {tuple(page_table.shape)}, expected [sequences, pages]")
+    return page_table.data_ptr()
+
+
+def _same_device(first: torch.Tensor, what: str, **others) -> None:
+    for name, t in others.items():
+        if t is not None and t.device != first.device:
+            raise KernelError(f"{what}: {name} is on {t.device}, not on {first.device}")
+    if first.is_cuda and first.device.index != torch.cuda.current_device():
+        raise KernelError(f"{what}: the tensors are on {first.device} but the current device is cuda:{torch.cuda.current_device()}")
+
+
+def kv4_prepare(qkv: torch.Tensor, wq: Optional[torch.Tensor], wk: Optional[torch.Tensor], eps: float,
+                inv_freq: Optional[torch.Tensor], half_split: bool, positions, seq_of, page_table, pool: torch.Tensor,
+                q_out: torch.Tensor, nh: int, nkv: int, hd: int) -> torch.Tensor:
+    """As :func:`qk_prepare`, into a cache held in 4 bits: per-head RMSNorm of q and k, rotation, and the write of k and v
+    as codes.  A row x (a token's key or value of one kv head) is held as zero = bf16(min x),
+    step = bf16(max(0, max x - zero) / 15) and the codes clamp(rint((x - zero) / step), 0, 15), and stands for
+    zero + step * code; a row with an element that is not finite stands for NaN throughout.  A (sequence, position) may
+    come once in a call.  ``pool``: uint8 [pages, kv heads, page_size * (hd + 8)]; of one kv head in one page the keys' codes
+    [row][hd / 2] (element d in byte d / 2, the even one in the low four bits), the values' codes, then (key step, key
+    zero, value step, value zero) bfloat16 [row][4]."""
+    N = qkv.shape[0]
+    page_size = _check_kv4(pool, nkv, hd, "kv4_prepare")
+    if nh < 1:
+        raise KernelError(f"kv4_prepare: {nh} heads")
+    for name, t in (("qkv", qkv), ("q norm weight", wq), ("k norm weight", wk)):
+        if t is not None and t.data_ptr() % 8:
+            raise KernelError(f"kv4_prepare: {name} must start on 8 bytes")
+    if q_out.data_ptr() % (2 * q_out.element_size()):
+        raise KernelError(f"kv4_prepare: q out must start on {2 * q_out.element_size()} bytes")
+    args = (_need(qkv, "qkv", torch.float32, (N, (nh + 2 * nkv) * hd)),
+            _need(wq, "q norm weight", torch.float32, (hd,), True), _need(wk, "k norm weight", torch.float32, (hd,), True),
+            float(eps), _need(inv_freq, "inv_freq", torch.float32, (hd // 2,), True), int(half_split),
+            _need(positions, "positions", torch.int32, (N,)), _need(seq_of, "seq_of", torch.int32, (N,)),
+            _check_table(page_table, "kv4_prepare"), page_table.shape[1], page_size, _need(pool, "cache pool"),
+            _need(q_out, "q out", None, (N, nh * hd)), _dt(q_out), N, nh, nkv, hd)
+    _same_device(qkv, "kv4_prepare", wq=wq, wk=wk, inv_freq=inv_freq, positions=positions, seq_of=seq_of, page_table=page_table,
+                 pool=pool, q_out=q_out)
+    _guard("core", "kv4_cache", qkv.device, n_pages=pool.shape[0])
+    _check(_fn("core", "mv_kv4_prepare")(*args, _stream()), "mv_kv4_prepare")
+    account(_nbytes(qkv, q_out) + N * nkv * (hd + 8))
+    return q_out
+
+
+def kv4_read(pool: torch.Tensor, page_table, positions, seq_of, k_out: torch.Tensor, v_out: torch.Tensor, nkv: int, hd: int):
+    """Rows of a cache held in 4 bits, read back: what the keys and values at ``positions`` [n] of the sequences ``seq_of`` [n]
+    (rows of the page table) stand for, into ``k_out`` and ``v_out`` [n, kv heads, head size], bfloat16 or float32."""
+    N = positions.shape[0]
+    page_size = _check_kv4(pool, nkv, hd, "kv4_read")
+    if k_out.dtype != v_out.dtype:
+        raise KernelError(f"kv4_read: k out is {k_out.dtype} but v out is {v_out.dtype}")
+    if k_out.data_ptr() % 16 or v_out.data_ptr() % 16:
+        raise KernelError("kv4_read: k out and v out must start on 16 bytes")
+    args = (_need(pool, "cache pool"), _check_table(page_table, "kv4_read"), page_table.shape[1], page_size,
+            _need(positions, "positions", torch.int32, (N,)), _need(seq_of, "seq_of", torch.int32, (N,)),
+            _need(k_out, "k out", None, (N, nkv, hd)), _need(v_out, "v out", None, (N, nkv, hd)), _dt(k_out), N, nkv, hd)
+    _same_device(pool, "kv4_read", page_table=page_table, positions=positions, seq_of=seq_of, k_out=k_out, v_out=v_out)
+    _guard("core", "kv4_cache", pool.device, n_pages=pool.shape[0])
+    _check(_fn("core", "mv_kv4_read")(*args, _stream()), "mv_kv4_read")
+    account(N * nkv * (hd + 8) + _nbytes(k_out, v_out))
+    return k_out, v_out
+
+
+KV4_DIRECT_TOKENS = 16              # tokens a sequence up to which a step's queries read the codes themselves
+KV4_READ_BYTES = 1 << 30            # most of the cache that is read back at a time, unless one sequence alone is more
+
+
+def kv4_runs(starts, lens, window: int, page_size: int, page_bytes: int):
+    """How a step's sequences are attended to: [(first sequence, one past the last, pages to read back, 0 for none)].  Neighbours
+    that bring at most ``KV4_DIRECT_TOKENS`` tokens each read the codes themselves, together; the others' pages (``page_bytes``
+    each once they are read back) are read back first, for as many neighbours together as ``KV4_READ_BYTES`` holds."""
+    runs = []
+    for b, (s, n) in enumerate(zip(starts, lens)):
+        pages = 0
+        if n > KV4_DIRECT_TOKENS:
+            first = max(0, s - window + 1) // page_size if window > 0 else 0
+            pages = -(-(s + n) // page_size) - first
+        if runs and (runs[-1][2] > 0) == (pages > 0) and (runs[-1][2] + pages) * page_bytes <= KV4_READ_BYTES:
+            runs[-1] = (runs[-1][0], b + 1, runs[-1][2] + pages)
+        else:
+            runs.append((b, b + 1, pages))
+    return runs
+
+
+def attention_kv4(q: torch.Tensor, pool: torch.Tensor, page_table, positions, seq_of, cu, starts, out: torch.Tensor, nh: int, nkv: int,
+                  hd: int, scale: float, window: int, ws, host_starts, host_lens, splits: Optional[int] = None) -> torch.Tensor:
+    """Causal attention of every token of the step over its sequence's cache held in 4 bits (which already holds the step's own
+    keys), optional sliding window: q and out [N, heads * head size] in bfloat16 or float32.  The step's tokens are packed sequence
+    by sequence (``cu``), sequence b bringing ``host_lens[b]`` tokens from position ``host_starts[b]`` = ``starts[b]`` on.  ``ws`` (a
+    Workspace) supplies the scratch; ``splits``: into how many parts the keys of single tokens are cut (None: by the step's
+    size and the page table's reach)."""
+    N, B = q.shape[0], len(host_lens)
+    page_size = _check_kv4(pool, nkv, hd, "attention_kv4")
+    if nh < 1 or nh % nkv:
+        raise KernelError(f"attention: {nh} heads are not a multiple of {nkv} kv heads")
+    if out.dtype != q.dtype:
+        raise KernelError(f"attention: q {q.dtype} and out {out.dtype} must agree")
+    if len(host_starts) != B or sum(host_lens) != N or (B and min(host_lens) < 1):
+        raise KernelError(f"attention_kv4: {len(host_starts)} starts and {B} lengths of {sum(host_lens)} tokens for {N} rows of q; every "
+                          "sequence brings a token or more")
+    if q.data_ptr() % 16 or out.data_ptr() % 16:
+        raise KernelError("attention_kv4: q and out must start on 16 bytes")
+    _dt(q)
+    _need(q, "q", None, (N, nh * hd))
+    _need(out, "attention out", None, (N, nh * hd))
+    _need(positions, "positions", torch.int32, (N,))
+    _need(seq_of, "seq_of", torch.int32, (N,))
+    _need(cu, "cu", torch.int32, (B + 1,))
+    _need(starts, "starts", torch.int32, (B,))
+    _need(pool, "cache pool")
+    _check_table(page_table, "attention_kv4")
+    if page_table.shape[0] < B:
+        raise KernelError(f"attention_kv4: a page table of {page_table.shape[0]} sequences for a step of {B}")
+    if B and max(s + n for s, n in zip(host_starts, host_lens)) > page_table.shape[1] * page_size:
+        raise KernelError(f"attention_kv4: {max(s + n for s, n in zip(host_starts, host_lens))} tokens in a sequence, the page table reaches "
+                          f"{page_table.shape[1] * page_size}")
+    _same_device(q, "attention_kv4", pool=pool, page_table=page_table, positions=positions, seq_of=seq_of, cu=cu, starts=starts, out=out)
+    n0 = 0
+    for b0, b1, pages in kv4_runs(host_starts, host_lens, window, page_size, 2 * nkv * page_size * hd * q.element_size()):
+        n1 = n0 + sum(host_lens[b0:b1])
+        if pages == 0:
+            _attention_kv4_direct(q[n0:n1], pool, page_table, page_size, positions[n0:n1], seq_of[n0:n1], out[n0:n1], nh, nkv, hd,
+                                  scale, window, ws, splits)
+        else:
+            _attention_kv4_pages(q, pool, page_table, page_size, positions, seq_of, cu, starts, out, b0, b1, n0, n1, pages, nh, nkv, hd,
+                                 scale, window, ws, host_lens)
+        n0 = n1
+    return out
+
+
+def attention_kv4_plan(N: int, nh: int, nkv: int, context_cap: int):
+    """(query heads per block, head tiles per kv head, key splits) of the CUDA-core kernel, in the manner of
+    ``attention_decode_plan``."""
+    G = nh // nkv
+    gt = 1 if G <= 1 else (2 if G <= 2 else 4)
+    head_tiles = -(-G // gt)
+    splits = -(-2 * n_sms() // max(1, N * nkv * head_tiles))
+    splits = max(splits, -(-context_cap // (32 * 4 * 8)))
+    return gt, head_tiles, max(1, min(32, splits))
+
+
+def _attention_kv4_direct(q, pool, page_table, page_size, positions, seq_of, out, nh, nkv, hd, scale, window, ws, splits):
+    N = q.shape[0]
+    gt, head_tiles, auto = attention_kv4_plan(N, nh, nkv, page_table.shape[1] * page_size)
+    splits = auto if splits is None else int(splits)
+    if not 1 <= splits <= 1024:
+        raise KernelError(f"attention_kv4: {splits} key splits, expected 1..1024")
+    if N > 65535 or nkv * head_tiles > 65535:
+        raise KernelError(f"attention_kv4: {N} tokens and {nkv} kv heads in one launch; each may be 65535 at most")
+    part_o = ws.get("attn_part_o", (N * nh * splits * hd,), torch.float32)
+    part_ml = ws.get("attn_part_ml", (N * nh * splits * 2,), torch.float32)
+    tickets = ws.get_zeroed("attn_tickets", (N * nkv * head_tiles,), torch.int32)
+    _guard("core", "kv4_cache", q.device, n_pages=pool.shape[0])
+    _check(_fn("core", "mv_attention_kv4")(
+        q.data_ptr(), pool.data_ptr(), page_table.data_ptr(), page_table.shape[1], page_size, positions.data_ptr(), seq_of.data_ptr(),
+        out.data_ptr(), _dt(q), part_o.data_ptr(), part_ml.data_ptr(), tickets.data_ptr(), N, nh, nkv, hd, float(scale), int(window),
+        splits, gt, head_tiles, _stream()), "mv_attention_kv4")
+
+
+def _attention_kv4_pages(q, pool, page_table, page_size, positions, seq_of, cu, starts, out, b0, b1, n0, n1, pages, nh, nkv, hd, scale,
+                         window, ws, host_lens):
+    """Sequences b0 .. b1 - 1: their pages are read back into a pool of their own, which the attention kernels of many tokens read."""
+    W, n_seqs = page_table.shape[1], b1 - b0
+    if n_seqs > 65535 or nkv > 65535:
+        raise KernelError(f"attention_kv4: {n_seqs} sequences and {nkv} kv heads in one launch; each may be 65535 at most")
+    # (a power of two pages: the pool keeps its shape, and with it its tensor map, as sequences grow)
+    read = ws.get("kv4_pages", (1 << (pages - 1).bit_length(), 2, nkv, page_size, hd), q.dtype)
+    table = ws.get("kv4_table", (page_table.shape[0], W), torch.int32)
+    cu_run, starts_run, table_run = cu[b0:b1 + 1], starts[b0:b1], table[b0:b1]
+    _guard("core", "kv4_cache", q.device, n_pages=pool.shape[0])
+    _check(_fn("core", "mv_kv4_read_pages")(
+        pool.data_ptr(), page_table[b0:b1].data_ptr(), W, page_size, cu_run.data_ptr(), starts_run.data_ptr(), int(window),
+        read.data_ptr(), _dt(read), table_run.data_ptr(), W, n_seqs, nkv, hd, _stream()), "mv_kv4_read_pages")
+    account(pages * nkv * page_size * (hd + 8 + 2 * hd * read.element_size()))
+    if n1 - n0 >= 128 * n_seqs and attention_prefill_tc_supported(q.dtype, hd, read, window):
+        attention_prefill_tc(q, read, table_run, cu_run, starts_run, out, n_seqs, nh, nkv, hd, scale)
+    elif attention_prefill_supported(q.dtype, hd):
+        attention_prefill(q, read, table_run, cu_run, starts_run, out, n_seqs, nh, nkv, hd, scale, window)
+    else:
+        attention_generic(q[n0:n1], read, table, positions[n0:n1], seq_of[n0:n1], out[n0:n1], nh, nkv, hd, scale, window,
+                          host_lens[b0:b1])
 
 
 def sample_scratch_width(V: int) -> int:

@@ -33,6 +33,9 @@ class Part:
     # instead of replaying a recorded CUDA graph.
     graph_safe = True
 
+    # True for a mixer whose keys and values may be held in 4 bits (its KVNeed then comes back with ``bits`` 4 in its view)
+    holds_4_bits = False
+
     def cache_need(self):
         """What this part keeps per sequence between steps: None, a KVNeed, a StateNeed, or a list of those."""
         return None

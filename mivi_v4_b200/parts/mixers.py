@@ -85,9 +85,11 @@ class GroupedQueryAttention(Part):
     1/sqrt(head_dim) and an optional window, out projection
     (crates/mivi-model/src/transformer.rs:55-110, 114-167, 304-350).
     ``shared_kv``: the layer has no k and v of its own and reads the cache of
-    another layer (its schedule entry says which)."""
+    another layer (its schedule entry says which).  Where the cache is held in 4 bits, k and v are quantised as they are
+    written, and every query, of this step's tokens too, sees what is held."""
 
     nested_roles = {"position": "position"}
+    holds_4_bits = True
 
     def __init__(self, hidden: int, n_heads: int, n_kv_heads: int, head_dim: int, position,
                  qk_norm_eps: Optional[float] = None, window: int = 0, shared_kv: bool = False):
@@ -147,7 +149,8 @@ class GroupedQueryAttention(Part):
         rot = self.position.rotary(u.device)
         inv_freq, half_split = rot if rot is not None else (None, False)
         eps = self.qk_norm_eps if self.qk_norm_eps is not None else 0.0
-        if not self.shared_kv and heads_fused_ok(N, u, self.w_qkv, hd, view.pool, half_split):
+        in_4_bits = view.need.bits == 4
+        if not self.shared_kv and not in_4_bits and heads_fused_ok(N, u, self.w_qkv, hd, view.pool, half_split):
             # a few tokens: norm, rotation and the append to the cache are the projection's epilogue
             linear_heads(u, self.w_qkv, self.q_norm, self.k_norm, eps, inv_freq, half_split, step.positions,
                          step.seq_of, view.page_table, view.pool, q, nh, nkv, scale=scale)
@@ -156,13 +159,19 @@ class GroupedQueryAttention(Part):
             linear(u, self.w_qkv, qkv, scale=scale)
             if self.shared_kv:
                 K.qk_prepare_q_only(qkv, self.q_norm, eps, inv_freq, half_split, step.positions, q, nh, hd)
+            elif in_4_bits:
+                K.kv4_prepare(qkv, self.q_norm, self.k_norm, eps, inv_freq, half_split, step.positions, step.seq_of,
+                              view.page_table, view.pool, q, nh, nkv, hd)
             else:
                 K.qk_prepare(qkv, self.q_norm, self.k_norm, eps, inv_freq, half_split, step.positions,
                              step.seq_of, view.page_table, view.pool, q, nh, nkv, hd)
         o = self.scratch(step, "mix", (N, nh * hd), step.dtype)
         # few query tokens, or many sequences with a token or two each: every query token on its own
         few = N <= K.DECODE_ATTENTION_MAX_TOKENS or step.max_len <= K.DECODE_ATTENTION_MAX_QUERIES
-        if few and K.attention_decode_tc_supported(step.dtype, hd, view.pool, self.window, nh, nkv):
+        if in_4_bits:
+            K.attention_kv4(q, view.pool, view.page_table, step.positions, step.seq_of, step.cu, step.starts, o, nh, nkv, hd,
+                            self.scale, self.window, step.ws, step.host_starts, step.host_lens)
+        elif few and K.attention_decode_tc_supported(step.dtype, hd, view.pool, self.window, nh, nkv):
             # few query tokens, head size 64: flash decoding with both products on tcgen05
             K.attention_decode_tc(q, view.pool, view.page_table, step.positions, step.seq_of, o, nh, nkv, hd,
                                   self.scale, step.ws)
@@ -183,8 +192,8 @@ class GroupedQueryAttention(Part):
             # keys that the step's queries read (each query its own context), for the attention launch
             pairs = sum(n * s + n * (n + 1) // 2 for s, n in zip(step.host_starts, step.host_lens))
             rows = pairs if few else sum(s + n for s, n in zip(step.host_starts, step.host_lens))
-            K.account(2 * nkv * hd * view.pool.element_size() * rows + 2 * N * nh * hd * q.element_size(),
-                      4 * nh * hd * pairs)
+            row = nkv * (hd + 8) if in_4_bits else 2 * nkv * hd * view.pool.element_size()
+            K.account(row * rows + 2 * N * nh * hd * q.element_size(), 4 * nh * hd * pairs)
         linear(o, self.w_o, resid, accumulate=True, emit=emit)
 
 

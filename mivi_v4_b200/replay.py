@@ -34,6 +34,8 @@ def main(argv: Optional[Sequence[str]] = None, stdin=None) -> int:
     ap.add_argument("--out", required=True, help="folder for <step>.f32 files")
     ap.add_argument("--max-tokens", type=int, required=True,
                     help="most tokens that live requests hold at any time")
+    ap.add_argument("--cache-dtype", default=None, choices=["int4"],
+                    help="int4: keys and values are held in 4 bits; default: in the model's dtype")
     args = ap.parse_args(argv)
 
     import torch
@@ -47,7 +49,7 @@ def main(argv: Optional[Sequence[str]] = None, stdin=None) -> int:
     # every live request may hold one page that is only partly filled, beyond the tokens it was counted for
     page_size, most_requests = 64, 256
     engine = Engine(model, max_tokens=max(page_size, args.max_tokens) + page_size * most_requests, max_batch=most_requests,
-                    page_size=page_size)
+                    page_size=page_size, cache_dtype=args.cache_dtype)
     slots = {}
     for line in (sys.stdin if stdin is None else stdin):
         line = line.strip()
