@@ -136,6 +136,7 @@ _SIGNATURES = {
                                      _P, _P],
         "mv_attention_decode_tc": [_P, _P, _Q, _P, _I, _P, _P, _P, _P, _P, _I, _I, _I, _F, _I, _P, _P],
         "mv_attention_prefill_tc": [_P, _P, _Q, _P, _I, _P, _P, _P, _I, _I, _I, _I, _F, _P, _P],
+        "mv_attention_kv4_decode": [_P, _P, _P, _I, _I, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _F, _I, _I, _I, _I, _I, _I, _P, _P],
         "mv_latent_attention_decode": [_P, _P, _Q, _P, _I, _I, _P, _P, _P, _P, _I, _I, _I, _I, _F, _I, _I, _P, _P, _P, _P],
         "mv_latent_query": [_P, _I, _I, _P, _P, _P, _I, _I, _I, _I, _I, _F, _P],
         "mv_latent_gather": [_P, _Q, _P, _I, _I, _P, _P, _I, _I, _I, _I, _P, _P, _I, _P],
@@ -2046,7 +2047,8 @@ _error_mirrors = {}
 # what a kernel's bounded waits put into the error flag when they run out: ranges of codes, a kernel each (4: a guarded index of any kernel)
 _ERROR_CODES = (((1, 3), "gemm_tc.cu"), ((5, 5), "gemm_tc.cu"), ((11, 21), "attention_prefill_tc.cu"), ((30, 40), "attention_decode_tc.cu"),
                 ((45, 45), "latent_attention_decode.cu"), ((51, 63), "latent_attention_tc.cu"), ((71, 76), "gemm_f32_tc.cu"),
-                ((81, 93), "attention_sink_tc.cu"), ((101, 103), "gemm_tc_swap.cu"), ((111, 115), "gemm_tc_pair.cu"))
+                ((81, 93), "attention_sink_tc.cu"), ((101, 103), "gemm_tc_swap.cu"), ((111, 115), "gemm_tc_pair.cu"),
+                ((150, 151), "attention_kv4_decode.cu"))
 # the products' roles, by the last digit
 _ERROR_ROLES = {1: "the TMA producer", 2: "the MMA issuer", 3: "the epilogue", 5: "the MMA issuer (for the epilogue)"}
 
@@ -2632,9 +2634,10 @@ def _check_kv4(pool: torch.Tensor, nkv: int, hd: int, what: str) -> int:
         raise KernelError(f"{what}: head size {hd} must be a multiple of 8 and at most {MAX_HEAD_DIM}")
     if nkv < 1:
         raise KernelError(f"{what}: {nkv} kv heads")
-    if pool.dtype != torch.uint8 or pool.dim() != 3 or pool.shape[1] != nkv or pool.shape[2] < 1 or pool.shape[2] % (hd + 8):
-        raise KernelError(f"{what}: a cache in 4 bits is uint8 [pages, {nkv}, page size * {hd + 8}], got {pool.dtype} {tuple(pool.shape)}")
-    page_size = pool.shape[2] // (hd + 8)
+    shape = pool.shape
+    if pool.dtype != torch.uint8 or len(shape) != 3 or shape[1] != nkv or shape[2] < 1 or shape[2] % (hd + 8):
+        raise KernelError(f"{what}: a cache in 4 bits is uint8 [pages, {nkv}, page size * {hd + 8}], got {pool.dtype} {tuple(shape)}")
+    page_size = shape[2] // (hd + 8)
     if page_size & (page_size - 1):
         raise KernelError(f"{what}: page size {page_size} is not a power of two")
     if pool.data_ptr() % 16:
@@ -2642,19 +2645,31 @@ def _check_kv4(pool: torch.Tensor, nkv: int, hd: int, what: str) -> int:
     return page_size
 
 
-def _check_table(page_table: torch.Tensor, what: str) -> int:
-    _need(page_table, "page table", torch.int32)
-    if page_table.dim() != 2 or page_table.shape[1] < 1:
-        raise KernelError(f"{what}: page table {tuple(page_table.shape)}, expected [sequences, pages]")
-    return page_table.data_ptr()
-
-
-def _same_device(first: torch.Tensor, what: str, **others) -> None:
-    for name, t in others.items():
+def _need_all(what: str, specs) -> int:
+    """``_need`` for [(name, tensor, dtype, shape)] at once, all on one device, the current one; returns its number.  One look
+    at each tensor while all is well (a call's checks take as long as its launch); what is wrong is worded by ``_need``."""
+    dev = specs[0][1].get_device()
+    for name, t, dtype, shape in specs:
+        if t is not None and (t.get_device() != dev or t.dtype != dtype or t.shape != shape or not t.is_contiguous()):
+            break
+    else:
+        if dev >= 0 and (_raw_device is None or _raw_device() == dev):
+            return dev
+    first = specs[0][1]
+    for name, t, dtype, shape in specs:
+        _need(t, name, dtype, shape, True)
         if t is not None and t.device != first.device:
             raise KernelError(f"{what}: {name} is on {t.device}, not on {first.device}")
-    if first.is_cuda and first.device.index != torch.cuda.current_device():
+    if first.device.index != torch.cuda.current_device():
         raise KernelError(f"{what}: the tensors are on {first.device} but the current device is cuda:{torch.cuda.current_device()}")
+    return first.device.index
+
+
+def _table_shape(page_table: torch.Tensor, what: str):
+    shape = page_table.shape
+    if len(shape) != 2 or shape[1] < 1:
+        raise KernelError(f"{what}: page table {tuple(shape)}, expected [sequences, pages]")
+    return shape
 
 
 def kv4_prepare(qkv: torch.Tensor, wq: Optional[torch.Tensor], wk: Optional[torch.Tensor], eps: float,
@@ -2671,22 +2686,24 @@ def kv4_prepare(qkv: torch.Tensor, wq: Optional[torch.Tensor], wk: Optional[torc
     page_size = _check_kv4(pool, nkv, hd, "kv4_prepare")
     if nh < 1:
         raise KernelError(f"kv4_prepare: {nh} heads")
-    for name, t in (("qkv", qkv), ("q norm weight", wq), ("k norm weight", wk)):
-        if t is not None and t.data_ptr() % 8:
-            raise KernelError(f"kv4_prepare: {name} must start on 8 bytes")
-    if q_out.data_ptr() % (2 * q_out.element_size()):
-        raise KernelError(f"kv4_prepare: q out must start on {2 * q_out.element_size()} bytes")
-    args = (_need(qkv, "qkv", torch.float32, (N, (nh + 2 * nkv) * hd)),
-            _need(wq, "q norm weight", torch.float32, (hd,), True), _need(wk, "k norm weight", torch.float32, (hd,), True),
-            float(eps), _need(inv_freq, "inv_freq", torch.float32, (hd // 2,), True), int(half_split),
-            _need(positions, "positions", torch.int32, (N,)), _need(seq_of, "seq_of", torch.int32, (N,)),
-            _check_table(page_table, "kv4_prepare"), page_table.shape[1], page_size, _need(pool, "cache pool"),
-            _need(q_out, "q out", None, (N, nh * hd)), _dt(q_out), N, nh, nkv, hd)
-    _same_device(qkv, "kv4_prepare", wq=wq, wk=wk, inv_freq=inv_freq, positions=positions, seq_of=seq_of, page_table=page_table,
-                 pool=pool, q_out=q_out)
+    table_shape = _table_shape(page_table, "kv4_prepare")
+    dt = _dt(q_out)
+    f32, i32 = torch.float32, torch.int32
+    _need_all("kv4_prepare", (("qkv", qkv, f32, (N, (nh + 2 * nkv) * hd)), ("q norm weight", wq, f32, (hd,)), ("k norm weight", wk, f32, (hd,)),
+                              ("inv_freq", inv_freq, f32, (hd // 2,)), ("positions", positions, i32, (N,)), ("seq_of", seq_of, i32, (N,)),
+                              ("page table", page_table, i32, table_shape), ("cache pool", pool, torch.uint8, pool.shape),
+                              ("q out", q_out, q_out.dtype, (N, nh * hd))))
+    ptr, out = qkv.data_ptr(), q_out.data_ptr()
+    wq_ptr, wk_ptr = None if wq is None else wq.data_ptr(), None if wk is None else wk.data_ptr()
+    for name, p in (("qkv", ptr), ("q out", out), ("q norm weight", wq_ptr or 0), ("k norm weight", wk_ptr or 0)):
+        if p % 16:
+            raise KernelError(f"kv4_prepare: {name} must start on 16 bytes")
     _guard("core", "kv4_cache", qkv.device, n_pages=pool.shape[0])
-    _check(_fn("core", "mv_kv4_prepare")(*args, _stream()), "mv_kv4_prepare")
-    account(_nbytes(qkv, q_out) + N * nkv * (hd + 8))
+    _check(_fn("core", "mv_kv4_prepare")(
+        ptr, wq_ptr, wk_ptr, eps, None if inv_freq is None else inv_freq.data_ptr(), bool(half_split), positions.data_ptr(), seq_of.data_ptr(),
+        page_table.data_ptr(), table_shape[1], page_size, pool.data_ptr(), out, dt, N, nh, nkv, hd, _stream()), "mv_kv4_prepare")
+    if _profile is not None:
+        account(_nbytes(qkv, q_out) + N * nkv * (hd + 8))
     return q_out
 
 
@@ -2697,15 +2714,18 @@ def kv4_read(pool: torch.Tensor, page_table, positions, seq_of, k_out: torch.Ten
     page_size = _check_kv4(pool, nkv, hd, "kv4_read")
     if k_out.dtype != v_out.dtype:
         raise KernelError(f"kv4_read: k out is {k_out.dtype} but v out is {v_out.dtype}")
-    if k_out.data_ptr() % 16 or v_out.data_ptr() % 16:
+    table_shape = _table_shape(page_table, "kv4_read")
+    dt, i32 = _dt(k_out), torch.int32
+    _need_all("kv4_read", (("cache pool", pool, torch.uint8, pool.shape), ("page table", page_table, i32, table_shape), ("positions", positions, i32, (N,)),
+                           ("seq_of", seq_of, i32, (N,)), ("k out", k_out, k_out.dtype, (N, nkv, hd)), ("v out", v_out, v_out.dtype, (N, nkv, hd))))
+    k_ptr, v_ptr = k_out.data_ptr(), v_out.data_ptr()
+    if k_ptr % 16 or v_ptr % 16:
         raise KernelError("kv4_read: k out and v out must start on 16 bytes")
-    args = (_need(pool, "cache pool"), _check_table(page_table, "kv4_read"), page_table.shape[1], page_size,
-            _need(positions, "positions", torch.int32, (N,)), _need(seq_of, "seq_of", torch.int32, (N,)),
-            _need(k_out, "k out", None, (N, nkv, hd)), _need(v_out, "v out", None, (N, nkv, hd)), _dt(k_out), N, nkv, hd)
-    _same_device(pool, "kv4_read", page_table=page_table, positions=positions, seq_of=seq_of, k_out=k_out, v_out=v_out)
     _guard("core", "kv4_cache", pool.device, n_pages=pool.shape[0])
-    _check(_fn("core", "mv_kv4_read")(*args, _stream()), "mv_kv4_read")
-    account(N * nkv * (hd + 8) + _nbytes(k_out, v_out))
+    _check(_fn("core", "mv_kv4_read")(pool.data_ptr(), page_table.data_ptr(), table_shape[1], page_size, positions.data_ptr(), seq_of.data_ptr(),
+                                      k_ptr, v_ptr, dt, N, nkv, hd, _stream()), "mv_kv4_read")
+    if _profile is not None:
+        account(N * nkv * (hd + 8) + _nbytes(k_out, v_out))
     return k_out, v_out
 
 
@@ -2746,36 +2766,38 @@ def attention_kv4(q: torch.Tensor, pool: torch.Tensor, page_table, positions, se
     if len(host_starts) != B or sum(host_lens) != N or (B and min(host_lens) < 1):
         raise KernelError(f"attention_kv4: {len(host_starts)} starts and {B} lengths of {sum(host_lens)} tokens for {N} rows of q; every "
                           "sequence brings a token or more")
+    if splits is not None and not 1 <= int(splits) <= 1024:
+        raise KernelError(f"attention_kv4: {splits} key splits, expected 1..1024")
+    dt, i32 = _dt(q), torch.int32
+    rows, W = table_shape = _table_shape(page_table, "attention_kv4")
+    dev = _need_all("attention_kv4", (("q", q, q.dtype, (N, nh * hd)), ("cache pool", pool, torch.uint8, pool.shape),
+                                      ("page table", page_table, i32, table_shape), ("positions", positions, i32, (N,)), ("seq_of", seq_of, i32, (N,)),
+                                      ("cu", cu, i32, (B + 1,)), ("starts", starts, i32, (B,)), ("attention out", out, q.dtype, (N, nh * hd))))
     if q.data_ptr() % 16 or out.data_ptr() % 16:
         raise KernelError("attention_kv4: q and out must start on 16 bytes")
-    _dt(q)
-    _need(q, "q", None, (N, nh * hd))
-    _need(out, "attention out", None, (N, nh * hd))
-    _need(positions, "positions", torch.int32, (N,))
-    _need(seq_of, "seq_of", torch.int32, (N,))
-    _need(cu, "cu", torch.int32, (B + 1,))
-    _need(starts, "starts", torch.int32, (B,))
-    _need(pool, "cache pool")
-    _check_table(page_table, "attention_kv4")
-    if page_table.shape[0] < B:
-        raise KernelError(f"attention_kv4: a page table of {page_table.shape[0]} sequences for a step of {B}")
-    if B and max(s + n for s, n in zip(host_starts, host_lens)) > page_table.shape[1] * page_size:
-        raise KernelError(f"attention_kv4: {max(s + n for s, n in zip(host_starts, host_lens))} tokens in a sequence, the page table reaches "
-                          f"{page_table.shape[1] * page_size}")
-    _same_device(q, "attention_kv4", pool=pool, page_table=page_table, positions=positions, seq_of=seq_of, cu=cu, starts=starts, out=out)
+    if B == 0:
+        return out
+    if rows < B:
+        raise KernelError(f"attention_kv4: a page table of {rows} sequences for a step of {B}")
+    max_len = max(host_lens)
+    if max(host_starts) + max_len > W * page_size and max(map(int.__add__, host_starts, host_lens)) > W * page_size:
+        raise KernelError(f"attention_kv4: {max(map(int.__add__, host_starts, host_lens))} tokens in a sequence, the page table reaches {W * page_size}")
+    args = (pool, page_table, page_size, positions, seq_of, starts, out, nh, nkv, hd, float(scale), int(window), ws)
+    if max_len <= KV4_DIRECT_TOKENS:
+        _attention_kv4_direct(q, *args, 0, N, max_len, splits, dt, dev)
+        return out
     n0 = 0
     for b0, b1, pages in kv4_runs(host_starts, host_lens, window, page_size, 2 * nkv * page_size * hd * q.element_size()):
         n1 = n0 + sum(host_lens[b0:b1])
         if pages == 0:
-            _attention_kv4_direct(q[n0:n1], pool, page_table, page_size, positions[n0:n1], seq_of[n0:n1], out[n0:n1], nh, nkv, hd,
-                                  scale, window, ws, splits)
+            _attention_kv4_direct(q, *args, n0, n1, max(host_lens[b0:b1]), splits, dt, dev)
         else:
-            _attention_kv4_pages(q, pool, page_table, page_size, positions, seq_of, cu, starts, out, b0, b1, n0, n1, pages, nh, nkv, hd,
-                                 scale, window, ws, host_lens)
+            _attention_kv4_pages(q, *args, cu, b0, b1, n0, n1, pages, host_lens)
         n0 = n1
     return out
 
 
+@functools.lru_cache(maxsize=4096)
 def attention_kv4_plan(N: int, nh: int, nkv: int, context_cap: int):
     """(query heads per block, head tiles per kv head, key splits) of the CUDA-core kernel, in the manner of
     ``attention_decode_plan``."""
@@ -2787,37 +2809,73 @@ def attention_kv4_plan(N: int, nh: int, nkv: int, context_cap: int):
     return gt, head_tiles, max(1, min(32, splits))
 
 
-def _attention_kv4_direct(q, pool, page_table, page_size, positions, seq_of, out, nh, nkv, hd, scale, window, ws, splits):
-    N = q.shape[0]
-    gt, head_tiles, auto = attention_kv4_plan(N, nh, nkv, page_table.shape[1] * page_size)
+def attention_kv4_decode_supported(dtype: torch.dtype, page_size: int) -> bool:
+    return dtype == torch.bfloat16 and page_size >= 16
+
+
+@functools.lru_cache(maxsize=4096)
+def attention_kv4_decode_plan(N: int, nh: int, nkv: int, hd: int, max_len: int, context_cap: int):
+    """(tiles of 8 query columns, head tiles per kv head, heads of a tile, tokens of a tile, key splits) for a step of N query tokens in
+    runs of at most ``max_len``.  A tile's columns are tokens by heads; more columns share a key's way from memory and into
+    operands, and cost registers.  Splits: enough blocks for four on each of the GPU's multiprocessors, and four tiles of
+    64 keys a block, one a warp.  Like ``attention_decode_plan`` it goes by the page table's reach, not by the lengths."""
+    G = nh // nkv
+    nt_max = 4 if hd <= 64 else 2 if hd <= 128 else 1
+    head_tiles = -(-G // (8 * nt_max))
+    heads = -(-G // head_tiles)
+    tokens = max(1, min(max_len, 8 * nt_max // heads)) if head_tiles == 1 else 1
+    nt = next(n for n in (1, 2, 4) if 8 * n >= heads * tokens)
+    if head_tiles == 1:
+        tokens = max(1, min(max_len, 8 * nt // heads))
+    blocks = -(-N // tokens) * nkv * head_tiles
+    splits = max(1, min(-(-4 * n_sms() // blocks), -(-context_cap // 256), 64))
+    return nt, head_tiles, heads, tokens, splits
+
+
+def _attention_kv4_direct(q, pool, page_table, page_size, positions, seq_of, starts, out, nh, nkv, hd, scale, window, ws, n0, n1, max_len, splits,
+                          dt, dev):
+    """The query rows n0 .. n1 - 1, in runs of at most ``max_len`` of a sequence, over the codes themselves."""
+    N, W = n1 - n0, page_table.shape[1]
+    tensor = dt == BF16 and page_size >= 16                      # attention_kv4_decode_supported
+    if tensor:
+        nt, head_tiles, heads, tokens, auto = attention_kv4_decode_plan(N, nh, nkv, hd, max_len, W * page_size)
+    else:
+        gt, head_tiles, auto = attention_kv4_plan(N, nh, nkv, W * page_size)
     splits = auto if splits is None else int(splits)
-    if not 1 <= splits <= 1024:
-        raise KernelError(f"attention_kv4: {splits} key splits, expected 1..1024")
     if N > 65535 or nkv * head_tiles > 65535:
         raise KernelError(f"attention_kv4: {N} tokens and {nkv} kv heads in one launch; each may be 65535 at most")
-    part_o = ws.get("attn_part_o", (N * nh * splits * hd,), torch.float32)
-    part_ml = ws.get("attn_part_ml", (N * nh * splits * 2,), torch.float32)
-    tickets = ws.get_zeroed("attn_tickets", (N * nkv * head_tiles,), torch.int32)
-    _guard("core", "kv4_cache", q.device, n_pages=pool.shape[0])
-    _check(_fn("core", "mv_attention_kv4")(
-        q.data_ptr(), pool.data_ptr(), page_table.data_ptr(), page_table.shape[1], page_size, positions.data_ptr(), seq_of.data_ptr(),
-        out.data_ptr(), _dt(q), part_o.data_ptr(), part_ml.data_ptr(), tickets.data_ptr(), N, nh, nkv, hd, float(scale), int(window),
-        splits, gt, head_tiles, _stream()), "mv_attention_kv4")
+    part_o = part_ml = tickets = None
+    if splits > 1:
+        part_o = ws.get("attn_part_o", (N * nh * splits * hd,), torch.float32).data_ptr()
+        part_ml = ws.get("attn_part_ml", (N * nh * splits * 2,), torch.float32).data_ptr()
+        tickets = ws.get_zeroed("attn_tickets", (N * nkv * head_tiles,), torch.int32).data_ptr()
+    row = nh * hd * (2 if dt == BF16 else 4) * n0
+    where = (q.data_ptr() + row, pool.data_ptr(), page_table.data_ptr(), W, page_size, positions.data_ptr() + 4 * n0, seq_of.data_ptr() + 4 * n0)
+    if tensor:
+        flag = _error_flags.get(dev)
+        _guard("bf16", "attention_kv4_decode", q.device, n_pages=pool.shape[0])
+        _check(_fn("bf16", "mv_attention_kv4_decode")(
+            *where, starts.data_ptr(), out.data_ptr() + row, part_o, part_ml, tickets, N, nh, nkv, hd, scale, window, splits, nt, head_tiles,
+            heads, tokens, (_error_flag(q.device) if flag is None else flag).data_ptr(), _stream()), "mv_attention_kv4_decode")
+    else:
+        _guard("core", "kv4_cache", q.device, n_pages=pool.shape[0])
+        _check(_fn("core", "mv_attention_kv4")(*where, out.data_ptr() + row, dt, part_o, part_ml, tickets, N, nh, nkv, hd, scale, window, splits, gt,
+                                               head_tiles, _stream()), "mv_attention_kv4")
 
 
-def _attention_kv4_pages(q, pool, page_table, page_size, positions, seq_of, cu, starts, out, b0, b1, n0, n1, pages, nh, nkv, hd, scale,
-                         window, ws, host_lens):
+def _attention_kv4_pages(q, pool, page_table, page_size, positions, seq_of, starts, out, nh, nkv, hd, scale, window, ws, cu, b0, b1, n0, n1, pages,
+                         host_lens):
     """Sequences b0 .. b1 - 1: their pages are read back into a pool of their own, which the attention kernels of many tokens read."""
     W, n_seqs = page_table.shape[1], b1 - b0
     if n_seqs > 65535 or nkv > 65535:
         raise KernelError(f"attention_kv4: {n_seqs} sequences and {nkv} kv heads in one launch; each may be 65535 at most")
     # (a power of two pages: the pool keeps its shape, and with it its tensor map, as sequences grow)
     read = ws.get("kv4_pages", (1 << (pages - 1).bit_length(), 2, nkv, page_size, hd), q.dtype)
-    table = ws.get("kv4_table", (page_table.shape[0], W), torch.int32)
+    table = ws.get("kv4_table", tuple(page_table.shape), torch.int32)
     cu_run, starts_run, table_run = cu[b0:b1 + 1], starts[b0:b1], table[b0:b1]
     _guard("core", "kv4_cache", q.device, n_pages=pool.shape[0])
     _check(_fn("core", "mv_kv4_read_pages")(
-        pool.data_ptr(), page_table[b0:b1].data_ptr(), W, page_size, cu_run.data_ptr(), starts_run.data_ptr(), int(window),
+        pool.data_ptr(), page_table.data_ptr() + 4 * W * b0, W, page_size, cu_run.data_ptr(), starts_run.data_ptr(), window,
         read.data_ptr(), _dt(read), table_run.data_ptr(), W, n_seqs, nkv, hd, _stream()), "mv_kv4_read_pages")
     account(pages * nkv * page_size * (hd + 8 + 2 * hd * read.element_size()))
     if n1 - n0 >= 128 * n_seqs and attention_prefill_tc_supported(q.dtype, hd, read, window):

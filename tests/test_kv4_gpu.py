@@ -478,7 +478,7 @@ def test_refusals_on_the_device():
             K().attention_kv4(**{**a, **over})
     with pytest.raises(KernelError, match="16 bytes"):
         K().kv4_read(pool, ints([[0]]), ints([0]), ints([0]), torch.zeros(nkv * hd + 1, device=DEV)[1:].view(1, nkv, hd), torch.zeros(1, nkv, hd, device=DEV), nkv, hd)
-    with pytest.raises(KernelError, match="8 bytes"):
+    with pytest.raises(KernelError, match="16 bytes"):
         K().kv4_prepare(torch.zeros((nh + 2 * nkv) * hd + 1, device=DEV)[1:].view(1, -1), None, None, 0.0, None, False, ints([0]), ints([0]), ints([[0]]), pool,
                         torch.zeros(1, nh * hd, device=DEV), nh, nkv, hd)
     # a step of nothing
