@@ -3,26 +3,35 @@
 //
 // What bounds it.  A key and its value of 64 elements are 72 bytes, so at the memory's rate a multiprocessor gets one every three clocks; in
 // that time it has to turn 128 codes into operands, score them and weight them.  The work goes by instructions issued, and the design counts
-// them: no element is ever worked out.  With x = zero + step * code = (zero + 8 step) + step * (code - 8),
-//     q.k = step_k * (q . (code_k - 8)) + (zero_k + 8 step_k) * sum(q)
+// them: no element of a row is ever worked out.  With x = zero + step * code,
+//     q.k = step_k (q . code_k) + zero_k sum(q)
 //     sum_t p_t v_t = sum_t (p_t step_t) (code_t - 8) + sum_t p_t (zero_t + 8 step_t)
-// so the products run on whole numbers from -8 to 7, which are exact in half precision and cost 1.2 instructions a pair to make (mask a
-// nibble pair into the mantissa of 1024 or 64, subtract), and the rows' numbers meet scores and weights, two an instruction.
+// so the products run on small whole numbers, and the rows' numbers meet scores and weights.
 //
-// Half precision, not bfloat16: its 11 bits hold a bfloat16 query exactly and give the weights eight times bfloat16's precision.  Its range
-// is small, so powers of two are taken out: of a query row its largest element's, of the weights p * step the largest step's so far
-// (weights whose step is 2^-24 of the largest vanish: so would their values beside the others' in bfloat16).
+// q . code: whole numbers, m16n8k32 of 8-bit operands.  A word of 8 codes becomes two operands in three instructions (mask the even nibbles,
+// shift, mask the odd ones).  A query is held as whole numbers of 16 bits, times a power of two of its own (its largest element has 15
+// or 16 of them, so what is lost is 2^-16 of that; a bfloat16 element within 2^-7 of it is exact), in two pieces of 8 bits that take
+// neighbouring columns: the 4 heads that usually share a kv head fill the 8 columns, and a lane's two accumulators are one score's two
+// pieces.  (In half precision a pair of codes costs 1.2 instructions each, twice the products, and half of the columns stay empty: 746
+// instructions a tile of 64 keys against some 480 now.)
 //
-// The scores are computed transposed, S^T = K Q^T, keys on the 16 rows of m16n8k16 and queries (tokens of one sequence x the heads that share
-// the kv head) on its 8 columns, so that the usual group of 4 heads fills half of a product and not a quarter.  Sums over K run over elements
-// in any order, so a lane takes a row's bytes as they lie (lane t of four: a quarter of the row) and reads its queries to match.  O^T = V^T
-// P^T likewise: a lane takes 8 neighbouring elements of four keys.  P^T gets from the accumulators' layout to the operand's by movmatrix.
+// Weights times values: m16n8k16 in half precision, whose 11 bits a weight needs (whole numbers of 15 bits lose those that lie far below the
+// largest).  Codes less 8 are exact in it and cost 1.25 instructions a code: merge two keys' words, mask a nibble of each into the mantissas
+// of 1024 or 64, subtract.  Half's range is small, so the weights p * step are taken relative to the largest step's power of two so far
+// (those whose step is 2^-24 of the largest vanish: so would their values beside the others' in bfloat16).
+//
+// The scores are computed transposed, S^T = K Q^T, keys on a product's 16 rows.  Sums over a row run over elements in any order, so a lane
+// takes the row's bytes as they lie (lane t of four: a quarter of it) and reads its queries to match.  O^T = V^T P^T: a lane takes 8
+// neighbouring elements of four keys.  P^T gets from the accumulators' layout to the operand's by movmatrix, two sets of 8 keys at a time:
+// they come out in the even and odd columns, and each set's product leaves the other's columns at 0, so a head's two columns add up.
 // Row r of a product is key r ^ (r >> 2 & 1) of its eight: with that order neither the keys' 8-byte nor the values' 4-byte shared loads of
 // rows of 32 bytes meet in a bank.
 //
-// Block = (tile of query columns, kv head, split of the keys), 4 warps, each with tiles of 64 keys of its own, STAGES ahead by bulk copies:
-// one of 4,608 bytes where a page has 64 rows, so that few instructions keep memory busy.  Warps merge in shared memory, splits in split
-// order by the block that finishes last (ticket counter, left at 0).
+// Block = (tile of query columns, kv head, piece of its keys), 4 warps, each with tiles of 64 keys of its own, STAGES ahead by bulk copies:
+// one of 4,608 bytes where a page has 64 rows, so that few instructions keep memory busy.  How long a piece is, and which piece a block
+// takes, is worked out on the device from the step's positions (a scan over its tokens): pieces of one length for all sequences, so many
+// that the device is filled.  So unequal sequences are balanced, and a recorded launch fits any lengths it is replayed with.  Warps merge
+// in shared memory, pieces in order by the block that finishes last (ticket counter, left at 0).
 #include "kv4.cuh"
 #include "tc_common.cuh"
 
@@ -38,9 +47,14 @@ __device__ __forceinline__ void bulk_load(unsigned dst, const void* src, unsigne
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
                  ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
 }
-__device__ __forceinline__ void mma16816(float (&d)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1) {
+__device__ __forceinline__ void mma_half(float (&d)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// unsigned by signed bytes
+__device__ __forceinline__ void mma_bytes(int (&d)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1) {
+    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ unsigned transpose8x8(unsigned a) {
     unsigned d;
@@ -61,43 +75,105 @@ __device__ __forceinline__ unsigned half_pair(float a, float b) {
 }
 __device__ __forceinline__ float pow2f(int e) { return __uint_as_float((unsigned)(e + 127) << 23); }       // e from -126 to 127
 
-// HDP: head size rounded up to 64, 128 or 256; NT: tiles of 8 query columns
+// HDP: head size rounded up to 64, 128 or 256; NT: tiles of 4 query columns (8 of a product)
 template <int HDP, int NT>
 struct KdShape {
+    static constexpr int RESIDENT = HDP == 64 ? (NT == 1 ? 4 : NT == 2 ? 3 : 2) : (HDP == 128 && NT == 1 ? 3 : 2);      // blocks a multiprocessor
     static constexpr int STAGES = HDP == 64 ? 3 : 2, STAGE_BYTES = KD_KEYS * (HDP + 8);
     // (the last row's loads of a head size below HDP reach past the stage)
-    static constexpr int RING = KD_WARPS * STAGES * STAGE_BYTES + HDP, MERGE = KD_WARPS * 8 * NT * (HDP + 4) * 4;
+    static constexpr int RING = KD_WARPS * STAGES * STAGE_BYTES + HDP, MERGE = KD_WARPS * 4 * NT * (HDP + 4) * 4;
     static constexpr int BARS = RING > MERGE ? RING : MERGE, SMEM = BARS + KD_WARPS * STAGES * 8;
 };
 
-// HDP: head size rounded up to 64, 128 or 256; EXACT: it is the head size.  NT: tiles of 8 query columns.  A column is token c / heads and
-// head h0 + c % heads of the kv head's group, heads = min(group, 8 NT); grid (splits, nkv * head_tiles, N); the block of a token whose
-// place in its sequence's run is no multiple of tokens_per_tile has nothing to do.
+// EXACT: HDP is the head size.  A column is token c / heads and head h0 + c % heads of the kv head's group, heads = min(group, 4 NT).  Only a token
+// whose place in its sequence's run is a multiple of tokens_per_tile begins a tile.  Block b works on kv head and head tile b % pairs of
+// piece b / pairs, counted over the tiles of columns.  piece: tiles of 64 keys in one, 0: such that there are ``blocks`` of them.
 template <int HDP, bool EXACT, int NT>
-__global__ void __launch_bounds__(KD_WARPS * 32, HDP == 64 ? (NT == 1 ? 4 : NT == 2 ? 3 : 2) : (HDP == 128 && NT == 1 ? 3 : 2))
+__global__ void __launch_bounds__(KD_WARPS * 32, KdShape<HDP, NT>::RESIDENT)
 attention_kv4_decode_kernel(const __nv_bfloat16* __restrict__ q, const unsigned char* __restrict__ pool, const int* __restrict__ page_table,
                             int table_stride, int page_shift, const int* __restrict__ positions, const int* __restrict__ seq_of,
                             const int* __restrict__ starts, __nv_bfloat16* __restrict__ o, float* __restrict__ part_o,
                             float* __restrict__ part_ml, int* __restrict__ tickets, int N, int nh, int nkv, int hd_, float scale_log2, int window,
-                            int head_tiles, int heads, int tokens_per_tile, int* __restrict__ err) {
+                            int head_tiles, int heads, int tokens_per_tile, int piece, int blocks, int* __restrict__ err) {
     mv_pdl_begin();
     using Shape = KdShape<HDP, NT>;
-    constexpr int STAGES = Shape::STAGES, COLS = 8 * NT, MT = HDP / 16, W = HDP / 32;      // W: words of a lane's quarter of a row
+    constexpr int STAGES = Shape::STAGES, COLS = 4 * NT, MT = HDP / 16, W = HDP / 32;      // W: words of a lane's quarter of a row
     extern __shared__ __align__(128) unsigned char smem[];
-    __shared__ int is_last;
+    __shared__ int scan[KD_WARPS], found[3], is_last;
     const int hd = EXACT ? HDP : hd_;
-    const int splits = gridDim.x, split = blockIdx.x, n = blockIdx.z;
-    const int kvh = blockIdx.y / head_tiles, h0 = (blockIdx.y - kvh * head_tiles) * heads;
-    const int group = nh / nkv, live_heads = min(heads, group - h0);
-    const int seq = seq_of[n], pos0 = positions[n];
-    int tokens = 1;
-    if (tokens_per_tile > 1) {
-        if ((pos0 - starts[seq]) % tokens_per_tile) return;
-        while (tokens < tokens_per_tile && n + tokens < N && seq_of[n + tokens] == seq) ++tokens;
+    const int warp = warp_index(), lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int pairs = nkv * head_tiles;
+
+    // ---- which tile of columns, which piece of its keys
+    // tokens that the tile of columns that begins with row r holds (0: none begins there), and its tiles of keys
+    auto tokens_at = [&](int r) {
+        if (tokens_per_tile == 1) return 1;
+        const int b = seq_of[r];
+        if ((positions[r] - starts[b]) % tokens_per_tile) return 0;
+        int k = 1;
+        while (k < tokens_per_tile && r + k < N && seq_of[r + k] == b) ++k;
+        return k;
+    };
+    auto tiles_at = [&](int r) {
+        const int k = r < N ? tokens_at(r) : 0;
+        if (k == 0) return 0;
+        const int p = positions[r];
+        return (p + k - 1) / KD_KEYS + 1 - (window > 0 ? max(0, p - window + 1) / KD_KEYS : 0);
+    };
+    auto block_sum = [&](int v, int& before) {                   // of one number a thread; before: of the threads before this one
+        int inc = v;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const int x = __shfl_up_sync(0xffffffffu, inc, d);
+            if (lane >= d) inc += x;
+        }
+        __syncthreads();
+        if (lane == 31) scan[warp] = inc;
+        __syncthreads();
+        int base = 0, all = 0;
+#pragma unroll
+        for (int w = 0; w < KD_WARPS; ++w) {
+            if (w < warp) base += scan[w];
+            all += scan[w];
+        }
+        before = base + inc - v;
+        return all;
+    };
+    int n, part, parts;
+    {
+        int before, mine = tiles_at(threadIdx.x);                // (of the first 128 rows; usually all there are)
+        if (piece == 0) {
+            long long all = block_sum(mine, before);
+            for (int r0 = KD_WARPS * 32; r0 < N; r0 += KD_WARPS * 32) all += block_sum(tiles_at(r0 + threadIdx.x), before);
+            // (half a piece a tile of columns is lost where its keys end: as many blocks are left to it)
+            const int aim = max(blocks / 2, blocks - (N * pairs + 1) / 2);
+            piece = max(KD_WARPS, (int)((all * pairs + aim - 1) / aim));
+        }
+        if (threadIdx.x == 0) found[0] = -1;
+        const int want = blockIdx.x / pairs;
+        int base = 0;
+        for (int r0 = 0; r0 < N && base <= want; r0 += KD_WARPS * 32) {
+            if (r0) mine = tiles_at(r0 + threadIdx.x);
+            const int count = (mine + piece - 1) / piece;
+            const int all = block_sum(count, before);
+            if (want >= base + before && want < base + before + count) {
+                found[0] = r0 + threadIdx.x;
+                found[1] = want - base - before;
+                found[2] = count;
+            }
+            base += all;
+        }
+        __syncthreads();
+        n = found[0];
+        part = found[1];
+        parts = found[2];
     }
+    if (n < 0) return;
+    const int pair = blockIdx.x % pairs, kvh = pair / head_tiles, h0 = (pair - kvh * head_tiles) * heads;
+    const int group = nh / nkv, live_heads = min(heads, group - h0);
+    const int seq = seq_of[n], pos0 = positions[n], tokens = tokens_at(n);
     const int pos_last = pos0 + tokens - 1, lo_key = window > 0 ? max(0, pos0 - window + 1) : 0;
     const int* table = page_table + (size_t)seq * table_stride;
-    const int warp = warp_index(), lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int page_size = 1 << page_shift;
     const size_t head_bytes = kv4_head_bytes(page_size, hd);
     const int stage_bytes = KD_KEYS * (hd + 8);
@@ -112,49 +188,53 @@ attention_kv4_decode_kernel(const __nv_bfloat16* __restrict__ q, const unsigned 
     }
     __syncwarp();
 
-    // this warp's tiles: every KD_WARPS-th of the split's
+    // this warp's tiles: every KD_WARPS-th of the piece's
     const int tile0 = lo_key / KD_KEYS, n_tiles = pos_last / KD_KEYS + 1 - tile0;
-    const int per = (n_tiles + splits - 1) / splits;
-    const int first = tile0 + split * per + warp, past = min(tile0 + n_tiles, tile0 + (split + 1) * per);
+    const int first = tile0 + part * piece + warp, past = tile0 + min(n_tiles, (part + 1) * piece);
     const int mine = first < past ? (past - first + KD_WARPS - 1) / KD_WARPS : 0;
-    auto fetch = [&](int i) {                                    // all lanes; lane 0 copies
+    // where the first page of a tile lies: asked for a tile early, so that the copy need not wait for the page table
+    auto page_of = [&](int i) { return i < mine ? mv_read_page(table[(first + i * KD_WARPS) * KD_KEYS >> page_shift]) : 0; };
+    auto fetch = [&](int i, int page) {                          // lane 0
         const int key0 = (first + i * KD_WARPS) * KD_KEYS;
-        if (lane == 0) {
-            const unsigned bar = bar0 + 8 * (i % STAGES), dst = ring + (i % STAGES) * Shape::STAGE_BYTES;
-            if (page_shift == 6) {
-                const int page = mv_read_page(table[key0 >> 6]);
-                mbar_expect_tx(bar, (unsigned)stage_bytes);
-                bulk_load(dst, pool + ((size_t)page * nkv + kvh) * head_bytes, (unsigned)stage_bytes, bar);
-            } else {
-                // rows a copy brings, and how many copies hold rows that exist
-                const int rows = min(KD_KEYS, page_size);
-                const int parts = min(KD_KEYS, pos_last + 1 - key0 + rows - 1) / rows;
-                mbar_expect_tx(bar, (unsigned)(parts * rows * (hd + 8)));
-                for (int p = 0; p < parts; ++p) {
-                    const int key = key0 + p * rows, row = key & (page_size - 1);
-                    // (behind a window, pages before the first key seen may be gone: their entry is a page all the same)
-                    const int page = mv_read_page(table[key >> page_shift]);
-                    const unsigned char* src = pool + ((size_t)page * nkv + kvh) * head_bytes;
-                    const unsigned codes = (unsigned)(rows * (hd >> 1));
-                    bulk_load(dst + p * codes, src + (size_t)row * (hd >> 1), codes, bar);
-                    bulk_load(dst + KD_KEYS * (hd >> 1) + p * codes, src + ((size_t)page_size + row) * (hd >> 1), codes, bar);
-                    bulk_load(dst + KD_KEYS * hd + p * rows * 8, src + (size_t)page_size * hd + (size_t)row * 8, (unsigned)(rows * 8), bar);
-                }
+        const unsigned bar = bar0 + 8 * (i % STAGES), dst = ring + (i % STAGES) * Shape::STAGE_BYTES;
+        const unsigned char* src = pool + ((size_t)page * nkv + kvh) * head_bytes;
+        if (page_shift == 6) {
+            mbar_expect_tx(bar, (unsigned)stage_bytes);
+            bulk_load(dst, src, (unsigned)stage_bytes, bar);
+        } else {
+            // rows a copy brings, and how many copies hold rows that exist
+            const int rows = min(KD_KEYS, page_size);
+            const int copies = min(KD_KEYS, pos_last + 1 - key0 + rows - 1) / rows;
+            const unsigned codes = (unsigned)(rows * (hd >> 1));
+            mbar_expect_tx(bar, (unsigned)(copies * rows * (hd + 8)));
+            for (int p = 0; p < copies; ++p) {
+                const int row = (key0 + p * rows) & (page_size - 1);
+                // (behind a window, pages before the first key seen may be gone: their entry is a page all the same)
+                if (p) src = pool + ((size_t)mv_read_page(table[(key0 + p * rows) >> page_shift]) * nkv + kvh) * head_bytes;
+                bulk_load(dst + p * codes, src + (size_t)row * (hd >> 1), codes, bar);
+                bulk_load(dst + KD_KEYS * (hd >> 1) + p * codes, src + ((size_t)page_size + row) * (hd >> 1), codes, bar);
+                bulk_load(dst + KD_KEYS * hd + p * rows * 8, src + (size_t)page_size * hd + (size_t)row * 8, (unsigned)(rows * 8), bar);
             }
         }
     };
-    for (int i = 0; i < min(mine, STAGES); ++i) fetch(i);
+#pragma unroll
+    for (int i = 0; i < STAGES; ++i)
+        if (i < mine) {
+            const int page = page_of(i);
+            if (lane == 0) fetch(i, page);
+        }
 
-    // queries: column 8 nt + g, elements of lane t's quarter of a row, in the order in which a word's nibbles come out
-    unsigned qf[NT][2 * W][2];
-    float2 lsc[NT], qsum[NT];                                    // of columns 2t and 2t + 1: factor to log2 units, sum of the row in them
-    int2 at_col[NT];                                             // and their positions (-1: no such column)
+    // Queries: of column 4 nt + g / 2 the high (g even) or low piece, elements of lane t's quarter of a row, the even and the odd ones of a word
+    unsigned qf[NT][W][2];
+    float lsc[NT], qsum[NT], unit[NT];                           // of column 4 nt + t: factor to log2 units, sum of the row and 1 in its units
+    int at_col[NT];                                              // and its position (-1: no such column)
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-        const int c = 8 * nt + g, tok = c / heads, h = c - tok * heads;
+        const int c = 4 * nt + (g >> 1), tok = c / heads, h = c - tok * heads;
         const bool live = tok < tokens && h < live_heads;
         const __nv_bfloat16* row = q + ((size_t)(n + (live ? tok : 0)) * nh + kvh * group + h0 + (live ? h : 0)) * hd;
-        float x[HDP / 4], top = 0.f, sum = 0.f;
+        float x[HDP / 4], top = 0.f;
+        bool fine = true;
 #pragma unroll
         for (int w = 0; w < W; ++w) {
             const int d = t * (HDP / 4) + 8 * w;
@@ -164,37 +244,58 @@ attention_kv4_decode_kernel(const __nv_bfloat16* __restrict__ q, const unsigned 
                 for (int e = 0; e < 8; ++e) x[8 * w + e] = 0.f;
         }
 #pragma unroll
-        for (int e = 0; e < HDP / 4; ++e) top = fmaxf(top, fabsf(x[e]));
+        for (int e = 0; e < HDP / 4; ++e) {
+            top = fmaxf(top, fabsf(x[e]));
+            fine = fine && fabsf(x[e]) < INFINITY;
+        }
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        const int ex = top > 0.f ? min(126, max(-126, (int)(__float_as_uint(top) >> 23) - 127)) : 0;
-        const float down = pow2f(-ex);
-#pragma unroll
-        for (int e = 0; e < HDP / 4; ++e) { x[e] *= down; sum += x[e]; }
-        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+        const unsigned quad = 0xfu << (lane & ~3);
+        fine = (__ballot_sync(0xffffffffu, fine) & quad) == quad;
+        // the largest element times 2^up: at least 2^13, and at most 127 * 256, so that its pieces are bytes
+        int up = top > 0.f && fine ? 14 - ((int)(__float_as_uint(top) >> 23) - 127) : 0;
+        if (top * pow2f(up >> 1) * pow2f(up - (up >> 1)) > 32512.f) --up;
+        const float up0 = pow2f(up >> 1), up1 = pow2f(up - (up >> 1));
+        int sum = 0;
 #pragma unroll
         for (int w = 0; w < W; ++w) {
-            qf[nt][2 * w][0] = half_pair(x[8 * w], x[8 * w + 4]);
-            qf[nt][2 * w][1] = half_pair(x[8 * w + 1], x[8 * w + 5]);
-            qf[nt][2 * w + 1][0] = half_pair(x[8 * w + 2], x[8 * w + 6]);
-            qf[nt][2 * w + 1][1] = half_pair(x[8 * w + 3], x[8 * w + 7]);
+#pragma unroll
+            for (int odd = 0; odd < 2; ++odd) {
+                unsigned bytes = 0u;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int v = fine ? __float2int_rn(x[8 * w + 2 * e + odd] * up0 * up1) : 0;
+                    const int low = ((v + 128) & 255) - 128;
+                    sum += v;
+                    bytes |= (unsigned)((g & 1 ? low : (v - low) >> 8) & 255) << (8 * e);
+                }
+                qf[nt][w][odd] = bytes;
+            }
         }
-        const float l = scale_log2 * pow2f(ex);
-        sum *= l;
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+        // A score is (q . code) step + sum(q) zero, below 2^25 times a row's numbers: for queries below 2^34 it is taken times 2^-30, so
+        // that rows near the largest floats do not pass them; larger ones meet rows so small that 2^-30 of their numbers would be lost.
+        const int spare = up > -20 ? -30 : 0;
+        const int ex = -up - spare;
+        const float f = fine ? scale_log2 * pow2f(max(-126, min(127, ex))) : NAN;
+        const float sm = (float)sum * pow2f(spare);
         const int at = live ? pos0 + tok : -1;
-        lsc[nt] = make_float2(__shfl_sync(0xffffffffu, l, 8 * t), __shfl_sync(0xffffffffu, l, 8 * t + 4));
-        qsum[nt] = make_float2(__shfl_sync(0xffffffffu, sum, 8 * t), __shfl_sync(0xffffffffu, sum, 8 * t + 4));
-        at_col[nt] = make_int2(__shfl_sync(0xffffffffu, at, 8 * t), __shfl_sync(0xffffffffu, at, 8 * t + 4));
+        // lane t scores column 4 nt + t, whose pieces lie in the lanes of g = 2t and 2t + 1
+        lsc[nt] = __shfl_sync(0xffffffffu, f, 8 * t);
+        qsum[nt] = __shfl_sync(0xffffffffu, sm, 8 * t);
+        unit[nt] = pow2f(__shfl_sync(0xffffffffu, spare, 8 * t));
+        at_col[nt] = __shfl_sync(0xffffffffu, at, 8 * t);
     }
 
     float oacc[NT][MT][4];
-    float2 m[NT], l[NT], pz[NT];                                 // maxima (log2 units, alike in all rows' lanes), this lane's sums
-    int ev = -126;                                               // the weights' power of two
+    float m[NT], l[NT], pz[NT];                                  // maxima (log2 units, alike in all rows' lanes), this lane's sums
+    int ev = -126;                                               // the weights' power of two, and its inverse
+    float ev_down = pow2f(126);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-        m[nt] = make_float2(-INFINITY, -INFINITY);
-        l[nt] = pz[nt] = make_float2(0.f, 0.f);
+        m[nt] = -INFINITY;
+        l[nt] = pz[nt] = 0.f;
 #pragma unroll
         for (int i = 0; i < MT; ++i)
 #pragma unroll
@@ -204,6 +305,7 @@ attention_kv4_decode_kernel(const __nv_bfloat16* __restrict__ q, const unsigned 
     const int vrow0 = (2 * t) ^ (t >> 1), vrow1 = (2 * t + 1) ^ (t >> 1);
     bool ok = true;
     for (int i = 0; i < mine; ++i) {
+        const int next_page = page_of(i + STAGES);
         ok = mbar_wait_warp(bar0 + 8 * (i % STAGES), (unsigned)(i / STAGES) & 1u, err, 150);
         if (!ok) {                                               // given up: the copies under way land before the block leaves
             for (int j = i + 1; j < min(mine, i + STAGES); ++j) mbar_wait_warp(bar0 + 8 * (j % STAGES), (unsigned)(j / STAGES) & 1u, err, 151);
@@ -213,20 +315,17 @@ attention_kv4_decode_kernel(const __nv_bfloat16* __restrict__ q, const unsigned 
         const unsigned char* vt = kt + KD_KEYS * (hd >> 1);
         const uint2* pt = reinterpret_cast<const uint2*>(kt + KD_KEYS * hd);
         const int key0 = (first + i * KD_WARPS) * KD_KEYS;
-        // every key of the tile is seen by every column (columns that stand for nothing may see what they like)
-        const bool whole = key0 + KD_KEYS - 1 <= pos0 && (window <= 0 || key0 > pos_last - window);
 
-        // ---- scores: 64 keys x 8 NT columns
-        float s[NT][4][4];
-        float zv[8];
-        float sv[8];
+        // ---- scores, in units of the columns' own: 64 keys x 4 NT columns; s[nt][r]: key 8 r + key_of
+        float s[NT][8], sv[8], zv[8];
         unsigned smax = 0u;
 #pragma unroll
         for (int b = 0; b < 4; ++b) {
+            int dot[NT][4];
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) s[nt][b][e] = 0.f;
+                for (int e = 0; e < 4; ++e) dot[nt][e] = 0;
             const unsigned char* r0 = kt + (16 * b + key_of) * (hd >> 1) + t * (HDP / 8);
             const unsigned char* r1 = r0 + 8 * (hd >> 1);
             unsigned w0[W], w1[W];
@@ -248,115 +347,141 @@ attention_kv4_decode_kernel(const __nv_bfloat16* __restrict__ q, const unsigned 
                 }
             }
 #pragma unroll
-            for (int w = 0; w < W; ++w) {
-                unsigned a0, a1, a2, a3;
-                centred(w0[w], a0, a2);
-                centred(w1[w], a1, a3);
+            for (int w = 0; w < W; ++w)
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) mma16816(s[nt][b], a0, a1, a2, a3, qf[nt][2 * w][0], qf[nt][2 * w][1]);
-                centred(w0[w] >> 8, a0, a2);
-                centred(w1[w] >> 8, a1, a3);
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) mma16816(s[nt][b], a0, a1, a2, a3, qf[nt][2 * w + 1][0], qf[nt][2 * w + 1][1]);
-            }
+                for (int nt = 0; nt < NT; ++nt)
+                    mma_bytes(dot[nt], w0[w] & 0x0f0f0f0fu, w1[w] & 0x0f0f0f0fu, (w0[w] >> 4) & 0x0f0f0f0fu, (w1[w] >> 4) & 0x0f0f0f0fu,
+                              qf[nt][w][0], qf[nt][w][1]);
 #pragma unroll
             for (int j = 0; j < 2; ++j) {                        // rows g and g + 8
-                const int key = 16 * b + 8 * j + key_of;
-                Kv4Params p = kv4_params(pt[key]);
-                kv4_poison(p);
-                const float kz = fmaf(8.f, p.ks, p.kz);
-                if (!whole && (key0 + key > pos_last || key0 + key < lo_key)) p.vs = p.vz = 0.f;
+                const Kv4Params p = kv4_params(pt[16 * b + 8 * j + key_of]);
                 sv[2 * b + j] = p.vs;
                 zv[2 * b + j] = fmaf(8.f, p.vs, p.vz);
                 smax = max(smax, __float_as_uint(p.vs));
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    // (the factors first: rows near the largest floats meet queries near the smallest)
-                    float2 y = fma2(make_float2(s[nt][b][2 * j], s[nt][b][2 * j + 1]), mul2(make_float2(p.ks, p.ks), lsc[nt]),
-                                    mul2(make_float2(kz, kz), qsum[nt]));
-                    if (!whole) {
-                        const int at = key0 + key;
-                        if (at > at_col[nt].x || (window > 0 && at <= at_col[nt].x - window)) y.x = -INFINITY;
-                        if (at > at_col[nt].y || (window > 0 && at <= at_col[nt].y - window)) y.y = -INFINITY;
-                    }
-                    s[nt][b][2 * j] = y.x;
-                    s[nt][b][2 * j + 1] = y.y;
-                }
+                for (int nt = 0; nt < NT; ++nt)
+                    s[nt][2 * b + j] = fmaf((float)(dot[nt][2 * j] * 256 + dot[nt][2 * j + 1]), p.ks * unit[nt], p.kz * qsum[nt]);
             }
         }
-        // ---- running maxima, the weights' power of two
+        // ---- at the edges: keys that some column, or none, sees
+        if (key0 + KD_KEYS - 1 > pos0 || (window > 0 && key0 <= pos_last - window)) {
+            smax = 0u;
+#pragma unroll
+            for (int r = 0; r < 8; ++r) {
+                const int at = key0 + 8 * r + key_of;
+                if (at > pos_last || at < lo_key) sv[r] = zv[r] = 0.f;
+                smax = max(smax, __float_as_uint(sv[r]));
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+                    if (at > at_col[nt] || (window > 0 && at <= at_col[nt] - window)) s[nt][r] = -INFINITY;
+            }
+        }
+        // ---- the weights' power of two
         smax = __reduce_max_sync(0xffffffffu, smax);
-        const int ev_new = max(ev, max(-126, (int)(smax >> 23) - 127));
-        const float ev_corr = ev_new == ev ? 1.f : (ev_new - ev > 126 ? 0.f : pow2f(ev - ev_new));
-        ev = ev_new;
-        const float down = pow2f(-ev);
+        if (smax > 0x7f7fffffu) {
+            // A value row that is not finite: whoever sees it gets a score that is not, and the row counts as 0 (0 * NaN would reach
+            // the columns that do not see it).
+            smax = 0u;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) sv[j] *= down;
-        float2 ref[NT];
+            for (int r = 0; r < 8; ++r) {
+                if (!(sv[r] < INFINITY)) {
+                    sv[r] = zv[r] = 0.f;
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-            float2 mx = m[nt];
-#pragma unroll
-            for (int b = 0; b < 4; ++b) {
-                mx.x = fmaxf(mx.x, fmaxf(s[nt][b][0], s[nt][b][2]));
-                mx.y = fmaxf(mx.y, fmaxf(s[nt][b][1], s[nt][b][3]));
-            }
-#pragma unroll
-            for (int d = 4; d < 32; d <<= 1) {
-                mx.x = fmaxf(mx.x, __shfl_xor_sync(0xffffffffu, mx.x, d));
-                mx.y = fmaxf(mx.y, __shfl_xor_sync(0xffffffffu, mx.y, d));
-            }
-            ref[nt] = make_float2(mx.x == -INFINITY ? 0.f : mx.x, mx.y == -INFINITY ? 0.f : mx.y);
-            const float2 corr = make_float2(m[nt].x == -INFINITY ? 0.f : ex2(m[nt].x - ref[nt].x), m[nt].y == -INFINITY ? 0.f : ex2(m[nt].y - ref[nt].y));
-            m[nt] = mx;
-            l[nt] = mul2(l[nt], corr);
-            pz[nt] = mul2(pz[nt], corr);
-            const float2 oc = mul2(corr, make_float2(ev_corr, ev_corr));
-            if (__any_sync(0xffffffffu, oc.x != 1.f || oc.y != 1.f))
-#pragma unroll
-                for (int k = 0; k < MT; ++k) {
-                    oacc[nt][k][0] *= oc.x; oacc[nt][k][1] *= oc.y;
-                    oacc[nt][k][2] *= oc.x; oacc[nt][k][3] *= oc.y;
+                    for (int nt = 0; nt < NT; ++nt)
+                        if (s[nt][r] != -INFINITY) s[nt][r] = NAN;
                 }
+                smax = max(smax, __float_as_uint(sv[r]));
+            }
+            smax = __reduce_max_sync(0xffffffffu, smax);
         }
-        // ---- weights and the values' product, 16 keys at a time
-#pragma unroll
-        for (int b = 0; b < 4; ++b) {
-            unsigned pb[NT][2];
+        const int ev_new = max(ev, (int)(smax >> 23) - 127);
+        if (ev_new != ev) {                                      // (as a rule only in the first tiles)
+            const float f = ev_new - ev > 126 ? 0.f : pow2f(ev - ev_new);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
+                for (int k = 0; k < MT; ++k)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) oacc[nt][k][e] *= f;
+            ev = ev_new;
+            ev_down = pow2f(-ev);
+        }
+        // ---- maxima: a column's reference moves when a score passes it by 2^8, for all columns of the warp together
+        bool moves = false;
+        float mx[NT];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            mx[nt] = s[nt][0];
+#pragma unroll
+            for (int r = 1; r < 8; ++r) mx[nt] = fmaxf(mx[nt], s[nt][r]);
+            mx[nt] *= lsc[nt];
+            moves = moves || mx[nt] > m[nt] + 8.f;
+        }
+        if (__any_sync(0xffffffffu, moves)) {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+                for (int d = 4; d < 32; d <<= 1) mx[nt] = fmaxf(mx[nt], __shfl_xor_sync(0xffffffffu, mx[nt], d));
+                mx[nt] = fmaxf(mx[nt], m[nt]);
+                const float corr = m[nt] == -INFINITY ? 0.f : ex2(m[nt] - mx[nt]);
+                m[nt] = mx[nt];
+                l[nt] *= corr;
+                pz[nt] *= corr;
+                // (a head's two columns of the accumulators are this lane's)
+#pragma unroll
+                for (int k = 0; k < MT; ++k)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) oacc[nt][k][e] *= corr;
+            }
+        }
+        // ---- weights and the values' product, 32 keys at a time
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+            unsigned pe[NT][2], po[NT][2];                       // even columns: the first 16 keys; odd ones: the second 16
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                const float ref = m[nt] == -INFINITY ? 0.f : -m[nt];        // (0 while a column has seen nothing: its weights come out as 0)
+#pragma unroll
                 for (int j = 0; j < 2; ++j) {
-                    const float2 y = make_float2(s[nt][b][2 * j] - ref[nt].x, s[nt][b][2 * j + 1] - ref[nt].y);
-                    const float2 p = make_float2(ex2(y.x), ex2(y.y));        // (ex2(-infinity) is 0: a key that is not seen)
-                    l[nt] = add2(l[nt], p);
-                    pz[nt] = fma2(p, make_float2(zv[2 * b + j], zv[2 * b + j]), pz[nt]);
-                    const float2 w = mul2(p, make_float2(sv[2 * b + j], sv[2 * b + j]));
-                    pb[nt][j] = transpose8x8(half_pair(w.x, w.y));
-                }
-            const unsigned char* v0 = vt + (16 * b + vrow0) * (hd >> 1) + 4 * g;
-            const unsigned char* v1 = vt + (16 * b + vrow1) * (hd >> 1) + 4 * g;
-#pragma unroll
-            for (int u = 0; u < HDP / 64; ++u) {
-                const unsigned wa = *reinterpret_cast<const unsigned*>(v0 + 32 * u), wb = *reinterpret_cast<const unsigned*>(v1 + 32 * u);
-                const unsigned wc = *reinterpret_cast<const unsigned*>(v0 + 8 * (hd >> 1) + 32 * u);
-                const unsigned wd = *reinterpret_cast<const unsigned*>(v1 + 8 * (hd >> 1) + 32 * u);
-#pragma unroll
-                for (int half = 0; half < 2; ++half) {           // elements 0 .. 3 of the lane's eight, then 4 .. 7
-                    const unsigned x0 = __byte_perm(wa, wb, half ? 0x7632 : 0x5410), x1 = __byte_perm(wc, wd, half ? 0x7632 : 0x5410);
+                    float w[2];
 #pragma unroll
                     for (int k = 0; k < 2; ++k) {
-                        unsigned a0, a1, a2, a3;
-                        centred(k ? x0 >> 8 : x0, a0, a1);
-                        centred(k ? x1 >> 8 : x1, a2, a3);
+                        const int r = 4 * b + 2 * k + j;
+                        const float p = ex2(fmaf(s[nt][r], lsc[nt], ref));  // (ex2(-infinity) is 0: a key that is not seen)
+                        l[nt] += p;
+                        pz[nt] = fmaf(p, zv[r], pz[nt]);
+                        w[k] = p * (sv[r] * ev_down);
+                    }
+                    const unsigned x = transpose8x8(half_pair(w[0], w[1]));
+                    pe[nt][j] = g & 1 ? 0u : x;
+                    po[nt][j] = g & 1 ? x : 0u;
+                }
+            }
 #pragma unroll
-                        for (int nt = 0; nt < NT; ++nt) mma16816(oacc[nt][4 * u + 2 * half + k], a0, a1, a2, a3, pb[nt][0], pb[nt][1]);
+            for (int k = 0; k < 2; ++k) {
+                const unsigned char* v0 = vt + (32 * b + 16 * k + vrow0) * (hd >> 1) + 4 * g;
+                const unsigned char* v1 = vt + (32 * b + 16 * k + vrow1) * (hd >> 1) + 4 * g;
+#pragma unroll
+                for (int u = 0; u < HDP / 64; ++u) {
+                    const unsigned wa = *reinterpret_cast<const unsigned*>(v0 + 32 * u), wb = *reinterpret_cast<const unsigned*>(v1 + 32 * u);
+                    const unsigned wc = *reinterpret_cast<const unsigned*>(v0 + 8 * (hd >> 1) + 32 * u);
+                    const unsigned wd = *reinterpret_cast<const unsigned*>(v1 + 8 * (hd >> 1) + 32 * u);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {                // elements 2 e and 2 e + 1 of the lane's eight
+                        const unsigned x0 = __byte_perm(wa, wb, e >> 1 ? 0x7632 : 0x5410) >> (e & 1 ? 8 : 0);
+                        const unsigned x1 = __byte_perm(wc, wd, e >> 1 ? 0x7632 : 0x5410) >> (e & 1 ? 8 : 0);
+                        unsigned a0, a1, a2, a3;
+                        centred(x0, a0, a1);
+                        centred(x1, a2, a3);
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt)
+                            mma_half(oacc[nt][4 * u + e], a0, a1, a2, a3, k ? po[nt][0] : pe[nt][0], k ? po[nt][1] : pe[nt][1]);
                     }
                 }
             }
         }
         __syncwarp();
-        if (i + STAGES < mine) fetch(i + STAGES);
+        if (lane == 0 && i + STAGES < mine) fetch(i + STAGES, next_page);
     }
 
     // ---- the warps' results meet in shared memory (in place of the rings)
@@ -369,26 +494,23 @@ attention_kv4_decode_kernel(const __nv_bfloat16* __restrict__ q, const unsigned 
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
         for (int d = 4; d < 32; d <<= 1) {
-            l[nt].x += __shfl_xor_sync(0xffffffffu, l[nt].x, d);
-            l[nt].y += __shfl_xor_sync(0xffffffffu, l[nt].y, d);
-            pz[nt].x += __shfl_xor_sync(0xffffffffu, pz[nt].x, d);
-            pz[nt].y += __shfl_xor_sync(0xffffffffu, pz[nt].y, d);
+            l[nt] += __shfl_xor_sync(0xffffffffu, l[nt], d);
+            pz[nt] += __shfl_xor_sync(0xffffffffu, pz[nt], d);
         }
-        const int c = 8 * nt + 2 * t;
+        const int c = 4 * nt + t;
         if (g == 0) {
-            xm[warp * COLS + c] = m[nt].x; xm[warp * COLS + c + 1] = m[nt].y;
-            xl[warp * COLS + c] = l[nt].x; xl[warp * COLS + c + 1] = l[nt].y;
+            xm[warp * COLS + c] = m[nt];
+            xl[warp * COLS + c] = l[nt];
         }
 #pragma unroll
         for (int u = 0; u < HDP / 64; ++u) {
-            float* d0 = xo + ((size_t)warp * COLS + c) * HDP + 64 * u + 8 * g;
-            float* d1 = d0 + HDP;
+            float* to = xo + ((size_t)warp * COLS + c) * HDP + 64 * u + 8 * g;
 #pragma unroll
             for (int k = 0; k < 4; k += 2) {
                 const float(&a)[4] = oacc[nt][4 * u + k];
                 const float(&b)[4] = oacc[nt][4 * u + k + 1];
-                *reinterpret_cast<float4*>(d0 + 2 * k) = make_float4(fmaf(a[0], up, pz[nt].x), fmaf(a[2], up, pz[nt].x), fmaf(b[0], up, pz[nt].x), fmaf(b[2], up, pz[nt].x));
-                *reinterpret_cast<float4*>(d1 + 2 * k) = make_float4(fmaf(a[1], up, pz[nt].y), fmaf(a[3], up, pz[nt].y), fmaf(b[1], up, pz[nt].y), fmaf(b[3], up, pz[nt].y));
+                *reinterpret_cast<float4*>(to + 2 * k) = make_float4(fmaf(a[0] + a[1], up, pz[nt]), fmaf(a[2] + a[3], up, pz[nt]),
+                                                                     fmaf(b[0] + b[1], up, pz[nt]), fmaf(b[2] + b[3], up, pz[nt]));
             }
         }
     }
@@ -412,19 +534,20 @@ attention_kv4_decode_kernel(const __nv_bfloat16* __restrict__ q, const unsigned 
             v.x = fmaf(x.x, f, v.x); v.y = fmaf(x.y, f, v.y); v.z = fmaf(x.z, f, v.z); v.w = fmaf(x.w, f, v.w);
         }
         const size_t row = (size_t)(n + tok) * nh + kvh * group + h0 + h;
-        if (splits == 1) {
+        if (parts == 1) {
             const float inv = 1.0f / L;
             mv_store4(o + row * hd + d, v.x * inv, v.y * inv, v.z * inv, v.w * inv);
         } else {
-            *reinterpret_cast<float4*>(part_o + (row * splits + split) * hd + d) = v;
-            if (d == 0) *reinterpret_cast<float2*>(part_ml + (row * splits + split) * 2) = make_float2(M, L);
+            const size_t at = (size_t)blockIdx.x * COLS + c;
+            *reinterpret_cast<float4*>(part_o + at * hd + d) = v;
+            if (d == 0) *reinterpret_cast<float2*>(part_ml + at * 2) = make_float2(M, L);
         }
     }
-    if (splits == 1) return;
+    if (parts == 1) return;
     __threadfence();
     __syncthreads();
-    int* ticket = tickets + (size_t)n * gridDim.y + blockIdx.y;
-    if (threadIdx.x == 0) is_last = atomicAdd(ticket, 1) == splits - 1;
+    int* ticket = tickets + (size_t)n * pairs + pair;
+    if (threadIdx.x == 0) is_last = atomicAdd(ticket, 1) == parts - 1;
     __syncthreads();
     if (!is_last) return;
     __threadfence();
@@ -432,12 +555,13 @@ attention_kv4_decode_kernel(const __nv_bfloat16* __restrict__ q, const unsigned 
         const int c0 = e / (hd >> 2), d = (e - c0 * (hd >> 2)) * 4;
         const int tok = c0 / live_heads, h = c0 - tok * live_heads;
         const size_t row = (size_t)(n + tok) * nh + kvh * group + h0 + h;
+        const size_t at0 = (size_t)(blockIdx.x - part * pairs) * COLS + tok * heads + h, step = (size_t)pairs * COLS;
         float M = -INFINITY, L = 0.f;
         float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int s = 0; s < splits; ++s) M = fmaxf(M, __ldcg(part_ml + (row * splits + s) * 2));
-        for (int s = 0; s < splits; ++s) {
-            const float2 ml = __ldcg(reinterpret_cast<const float2*>(part_ml + (row * splits + s) * 2));
-            const float4 x = __ldcg(reinterpret_cast<const float4*>(part_o + (row * splits + s) * hd + d));
+        for (int s = 0; s < parts; ++s) M = fmaxf(M, __ldcg(part_ml + (at0 + s * step) * 2));
+        for (int s = 0; s < parts; ++s) {
+            const float2 ml = __ldcg(reinterpret_cast<const float2*>(part_ml + (at0 + s * step) * 2));
+            const float4 x = __ldcg(reinterpret_cast<const float4*>(part_o + (at0 + s * step) * hd + d));
             const float f = share(ml.x, ml.y, M);
             L = fmaf(ml.y, f, L);
             v.x = fmaf(x.x, f, v.x); v.y = fmaf(x.y, f, v.y); v.z = fmaf(x.z, f, v.z); v.w = fmaf(x.w, f, v.w);
@@ -459,26 +583,26 @@ int kd_launch(dim3 grid, cudaStream_t stream, A... args) {
 
 }  // namespace
 
-// bfloat16; pages of 16 rows or more.  nt: tiles of 8 query columns, 1, 2 or 4 (2 at most above heads of 64, 1 above 128).  A tile of columns is
-// tokens_per_tile consecutive tokens of one sequence by ``heads`` heads of a kv head's group (tokens_per_tile * heads <= 8 nt; several tokens
-// only where heads is the whole group).  part_o [N, nh, splits, hd], part_ml [N, nh, splits, 2] and tickets [N, nkv * head_tiles] (zero)
-// are used with splits > 1.
+// bfloat16; pages of 16 rows or more.  nt: tiles of 4 query columns, 1, 2 or 4 (2 at most above heads of 128).  A tile of columns is
+// tokens_per_tile consecutive tokens of one sequence by ``heads`` heads of a kv head's group (tokens_per_tile * heads <= 4 nt; several tokens
+// only where heads is the whole group).  The keys are cut into pieces of ``piece`` tiles of 64 (0: such that there are about ``blocks``
+// pieces in all); ``grid`` bounds the pieces times kv heads and head tiles: blocks + N * nkv * head_tiles where piece is 0.
+// part_o [grid, 4 nt, hd] and part_ml [grid, 4 nt, 2] float32, tickets [N, nkv * head_tiles] (zero).
 MV_API int mv_attention_kv4_decode(const void* q, const void* pool, const int* page_table, int table_stride, int page_size,
                                    const int* positions, const int* seq_of, const int* starts, void* o, float* part_o, float* part_ml,
-                                   int* tickets, int N, int nh, int nkv, int hd, float scale, int window, int splits, int nt, int head_tiles,
-                                   int heads, int tokens_per_tile, int* err, cudaStream_t stream) {
+                                   int* tickets, int N, int nh, int nkv, int hd, float scale, int window, int nt, int head_tiles, int heads,
+                                   int tokens_per_tile, int piece, int blocks, int grid, int* err, cudaStream_t stream) {
     if (N <= 0) return 0;
-    if (hd % 8 || hd < 8 || hd > KV4_MAX_HEAD_DIM || nkv < 1 || nh % nkv || page_size < 16 || (page_size & (page_size - 1)) || splits < 1 ||
-        N > 65535 || nkv * head_tiles > 65535 || heads < 1 || heads * head_tiles < nh / nkv || tokens_per_tile < 1 ||
-        heads * tokens_per_tile > 8 * nt || (tokens_per_tile > 1 && head_tiles > 1) || ((uintptr_t)pool & 15))
+    if (hd % 8 || hd < 8 || hd > KV4_MAX_HEAD_DIM || nkv < 1 || nh % nkv || page_size < 16 || (page_size & (page_size - 1)) || blocks < 1 ||
+        grid < 1 || piece < 0 || heads < 1 || heads * head_tiles < nh / nkv || tokens_per_tile < 1 ||
+        heads * tokens_per_tile > 4 * nt || (tokens_per_tile > 1 && head_tiles > 1) || ((uintptr_t)pool & 15))
         return (int)cudaErrorInvalidValue;
     int page_shift = 0;
     while ((1 << page_shift) < page_size) ++page_shift;
-    const dim3 grid(splits, nkv * head_tiles, N);
 #define MV_GO(HDP, EXACT, NT)                                                                                                            \
-    return kd_launch<HDP, EXACT, NT>(grid, stream, (const __nv_bfloat16*)q, (const unsigned char*)pool, page_table, table_stride, page_shift, \
-                                     positions, seq_of, starts, (__nv_bfloat16*)o, part_o, part_ml, tickets, N, nh, nkv, hd,              \
-                                     scale * 1.4426950408889634f, window, head_tiles, heads, tokens_per_tile, err)
+    return kd_launch<HDP, EXACT, NT>(dim3(grid), stream, (const __nv_bfloat16*)q, (const unsigned char*)pool, page_table, table_stride,   \
+                                     page_shift, positions, seq_of, starts, (__nv_bfloat16*)o, part_o, part_ml, tickets, N, nh, nkv, hd,  \
+                                     scale * 1.4426950408889634f, window, head_tiles, heads, tokens_per_tile, piece, blocks, err)
     if (hd <= 64) {
         if (hd == 64) {
             if (nt == 1) MV_GO(64, true, 1);
@@ -493,13 +617,18 @@ MV_API int mv_attention_kv4_decode(const void* q, const void* pool, const int* p
         if (hd == 128) {
             if (nt == 1) MV_GO(128, true, 1);
             if (nt == 2) MV_GO(128, true, 2);
+            if (nt == 4) MV_GO(128, true, 4);
         } else {
             if (nt == 1) MV_GO(128, false, 1);
             if (nt == 2) MV_GO(128, false, 2);
+            if (nt == 4) MV_GO(128, false, 4);
         }
-    } else if (nt == 1) {
-        if (hd == 256) MV_GO(256, true, 1);
-        MV_GO(256, false, 1);
+    } else if (hd == 256) {
+        if (nt == 1) MV_GO(256, true, 1);
+        if (nt == 2) MV_GO(256, true, 2);
+    } else {
+        if (nt == 1) MV_GO(256, false, 1);
+        if (nt == 2) MV_GO(256, false, 2);
     }
 #undef MV_GO
     return (int)cudaErrorInvalidValue;

@@ -136,7 +136,7 @@ _SIGNATURES = {
                                      _P, _P],
         "mv_attention_decode_tc": [_P, _P, _Q, _P, _I, _P, _P, _P, _P, _P, _I, _I, _I, _F, _I, _P, _P],
         "mv_attention_prefill_tc": [_P, _P, _Q, _P, _I, _P, _P, _P, _I, _I, _I, _I, _F, _P, _P],
-        "mv_attention_kv4_decode": [_P, _P, _P, _I, _I, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _F, _I, _I, _I, _I, _I, _I, _P, _P],
+        "mv_attention_kv4_decode": [_P, _P, _P, _I, _I, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _F, _I, _I, _I, _I, _I, _I, _I, _I, _P, _P],
         "mv_latent_attention_decode": [_P, _P, _Q, _P, _I, _I, _P, _P, _P, _P, _I, _I, _I, _I, _F, _I, _I, _P, _P, _P, _P],
         "mv_latent_query": [_P, _I, _I, _P, _P, _P, _I, _I, _I, _I, _I, _F, _P],
         "mv_latent_gather": [_P, _Q, _P, _I, _I, _P, _P, _I, _I, _I, _I, _P, _P, _I, _P],
@@ -2755,8 +2755,8 @@ def attention_kv4(q: torch.Tensor, pool: torch.Tensor, page_table, positions, se
     """Causal attention of every token of the step over its sequence's cache held in 4 bits (which already holds the step's own
     keys), optional sliding window: q and out [N, heads * head size] in bfloat16 or float32.  The step's tokens are packed sequence
     by sequence (``cu``), sequence b bringing ``host_lens[b]`` tokens from position ``host_starts[b]`` = ``starts[b]`` on.  ``ws`` (a
-    Workspace) supplies the scratch; ``splits``: into how many parts the keys of single tokens are cut (None: by the step's
-    size and the page table's reach)."""
+    Workspace) supplies the scratch; ``splits``: into how many parts the longest sequence's keys are cut where the codes are read
+    (None: as fills the device)."""
     N, B = q.shape[0], len(host_lens)
     page_size = _check_kv4(pool, nkv, hd, "attention_kv4")
     if nh < 1 or nh % nkv:
@@ -2766,6 +2766,8 @@ def attention_kv4(q: torch.Tensor, pool: torch.Tensor, page_table, positions, se
     if len(host_starts) != B or sum(host_lens) != N or (B and min(host_lens) < 1):
         raise KernelError(f"attention_kv4: {len(host_starts)} starts and {B} lengths of {sum(host_lens)} tokens for {N} rows of q; every "
                           "sequence brings a token or more")
+    if not 0.0 < scale < 1e4:
+        raise KernelError(f"attention_kv4: scale {scale}, expected a positive number")
     if splits is not None and not 1 <= int(splits) <= 1024:
         raise KernelError(f"attention_kv4: {splits} key splits, expected 1..1024")
     dt, i32 = _dt(q), torch.int32
@@ -2784,13 +2786,13 @@ def attention_kv4(q: torch.Tensor, pool: torch.Tensor, page_table, positions, se
         raise KernelError(f"attention_kv4: {max(map(int.__add__, host_starts, host_lens))} tokens in a sequence, the page table reaches {W * page_size}")
     args = (pool, page_table, page_size, positions, seq_of, starts, out, nh, nkv, hd, float(scale), int(window), ws)
     if max_len <= KV4_DIRECT_TOKENS:
-        _attention_kv4_direct(q, *args, 0, N, max_len, splits, dt, dev)
+        _attention_kv4_direct(q, *args, 0, N, max_len, max(host_starts) + max_len, splits, dt, dev)
         return out
     n0 = 0
     for b0, b1, pages in kv4_runs(host_starts, host_lens, window, page_size, 2 * nkv * page_size * hd * q.element_size()):
         n1 = n0 + sum(host_lens[b0:b1])
         if pages == 0:
-            _attention_kv4_direct(q, *args, n0, n1, max(host_lens[b0:b1]), splits, dt, dev)
+            _attention_kv4_direct(q, *args, n0, n1, max(host_lens[b0:b1]), max(host_starts) + max_len, splits, dt, dev)
         else:
             _attention_kv4_pages(q, *args, cu, b0, b1, n0, n1, pages, host_lens)
         n0 = n1
@@ -2813,34 +2815,55 @@ def attention_kv4_decode_supported(dtype: torch.dtype, page_size: int) -> bool:
     return dtype == torch.bfloat16 and page_size >= 16
 
 
+KV4_DECODE_WAVES = 1                # how many times over the pieces of a step fill the device
+
+
 @functools.lru_cache(maxsize=4096)
-def attention_kv4_decode_plan(N: int, nh: int, nkv: int, hd: int, max_len: int, context_cap: int):
-    """(tiles of 8 query columns, head tiles per kv head, heads of a tile, tokens of a tile, key splits) for a step of N query tokens in
-    runs of at most ``max_len``.  A tile's columns are tokens by heads; more columns share a key's way from memory and into
-    operands, and cost registers.  Splits: enough blocks for four on each of the GPU's multiprocessors, and four tiles of
-    64 keys a block, one a warp.  Like ``attention_decode_plan`` it goes by the page table's reach, not by the lengths."""
+def attention_kv4_decode_plan(N: int, nh: int, nkv: int, hd: int, max_len: int):
+    """(tiles of 4 query columns, head tiles per kv head, heads of a tile, tokens of a tile, blocks aimed at) for a step of N query tokens
+    in runs of at most ``max_len``.  A tile's columns are tokens by heads; more columns share a key's way from memory and into
+    operands, and cost registers.  The kernel cuts the keys into equal pieces by the lengths that it finds."""
     G = nh // nkv
-    nt_max = 4 if hd <= 64 else 2 if hd <= 128 else 1
-    head_tiles = -(-G // (8 * nt_max))
+    nt_max = 4 if hd <= 128 else 2
+    head_tiles = -(-G // (4 * nt_max))
     heads = -(-G // head_tiles)
-    tokens = max(1, min(max_len, 8 * nt_max // heads)) if head_tiles == 1 else 1
-    nt = next(n for n in (1, 2, 4) if 8 * n >= heads * tokens)
+    tokens = max(1, min(max_len, 4 * nt_max // heads)) if head_tiles == 1 else 1
+    nt = next(n for n in (1, 2, 4) if 4 * n >= heads * tokens)
     if head_tiles == 1:
-        tokens = max(1, min(max_len, 8 * nt // heads))
-    blocks = -(-N // tokens) * nkv * head_tiles
-    splits = max(1, min(-(-4 * n_sms() // blocks), -(-context_cap // 256), 64))
-    return nt, head_tiles, heads, tokens, splits
+        tokens = max(1, min(max_len, 4 * nt // heads))
+    resident = {1: 4, 2: 3, 4: 2}[nt] if hd <= 64 else 3 if hd <= 128 and nt == 1 else 2       # blocks on a multiprocessor (KdShape)
+    return nt, head_tiles, heads, tokens, KV4_DECODE_WAVES * resident * n_sms()
 
 
-def _attention_kv4_direct(q, pool, page_table, page_size, positions, seq_of, starts, out, nh, nkv, hd, scale, window, ws, n0, n1, max_len, splits,
-                          dt, dev):
-    """The query rows n0 .. n1 - 1, in runs of at most ``max_len`` of a sequence, over the codes themselves."""
+def _attention_kv4_direct(q, pool, page_table, page_size, positions, seq_of, starts, out, nh, nkv, hd, scale, window, ws, n0, n1, max_len, reach,
+                          splits, dt, dev):
+    """The query rows n0 .. n1 - 1, in runs of at most ``max_len`` of a sequence, over the codes themselves.  ``reach``: rows of the
+    longest sequence."""
     N, W = n1 - n0, page_table.shape[1]
-    tensor = dt == BF16 and page_size >= 16                      # attention_kv4_decode_supported
-    if tensor:
-        nt, head_tiles, heads, tokens, auto = attention_kv4_decode_plan(N, nh, nkv, hd, max_len, W * page_size)
-    else:
-        gt, head_tiles, auto = attention_kv4_plan(N, nh, nkv, W * page_size)
+    row = nh * hd * (2 if dt == BF16 else 4) * n0
+    where = (q.data_ptr() + row, pool.data_ptr(), page_table.data_ptr(), W, page_size, positions.data_ptr() + 4 * n0, seq_of.data_ptr() + 4 * n0)
+    if dt == BF16 and page_size >= 16:                           # attention_kv4_decode_supported
+        nt, head_tiles, heads, tokens, blocks = attention_kv4_decode_plan(N, nh, nkv, hd, max_len)
+        pairs, piece = nkv * head_tiles, 0
+        grid = blocks + N * pairs
+        if splits is not None:
+            piece = -(-(-(-reach // 64)) // int(splits))
+            grid = N * pairs * (-(-(reach // 64 + 2) // piece))
+        elif W * page_size <= 256:                               # one piece is all there can be
+            grid = N * pairs
+        if grid > 0x7fffffff:
+            raise KernelError(f"attention_kv4: {N} tokens and {nkv} kv heads make {grid} blocks")
+        part_o = ws.get("attn_part_o", (grid * 4 * nt * hd,), torch.float32)
+        part_ml = ws.get("attn_part_ml", (grid * 4 * nt * 2,), torch.float32)
+        tickets = ws.get_zeroed("attn_tickets", (N * pairs,), torch.int32)
+        flag = _error_flags.get(dev)
+        _guard("bf16", "attention_kv4_decode", q.device, n_pages=pool.shape[0])
+        _check(_fn("bf16", "mv_attention_kv4_decode")(
+            *where, starts.data_ptr(), out.data_ptr() + row, part_o.data_ptr(), part_ml.data_ptr(), tickets.data_ptr(), N, nh, nkv, hd, scale,
+            window, nt, head_tiles, heads, tokens, piece, blocks, grid, (_error_flag(q.device) if flag is None else flag).data_ptr(), _stream()),
+            "mv_attention_kv4_decode")
+        return
+    gt, head_tiles, auto = attention_kv4_plan(N, nh, nkv, W * page_size)
     splits = auto if splits is None else int(splits)
     if N > 65535 or nkv * head_tiles > 65535:
         raise KernelError(f"attention_kv4: {N} tokens and {nkv} kv heads in one launch; each may be 65535 at most")
@@ -2849,18 +2872,9 @@ def _attention_kv4_direct(q, pool, page_table, page_size, positions, seq_of, sta
         part_o = ws.get("attn_part_o", (N * nh * splits * hd,), torch.float32).data_ptr()
         part_ml = ws.get("attn_part_ml", (N * nh * splits * 2,), torch.float32).data_ptr()
         tickets = ws.get_zeroed("attn_tickets", (N * nkv * head_tiles,), torch.int32).data_ptr()
-    row = nh * hd * (2 if dt == BF16 else 4) * n0
-    where = (q.data_ptr() + row, pool.data_ptr(), page_table.data_ptr(), W, page_size, positions.data_ptr() + 4 * n0, seq_of.data_ptr() + 4 * n0)
-    if tensor:
-        flag = _error_flags.get(dev)
-        _guard("bf16", "attention_kv4_decode", q.device, n_pages=pool.shape[0])
-        _check(_fn("bf16", "mv_attention_kv4_decode")(
-            *where, starts.data_ptr(), out.data_ptr() + row, part_o, part_ml, tickets, N, nh, nkv, hd, scale, window, splits, nt, head_tiles,
-            heads, tokens, (_error_flag(q.device) if flag is None else flag).data_ptr(), _stream()), "mv_attention_kv4_decode")
-    else:
-        _guard("core", "kv4_cache", q.device, n_pages=pool.shape[0])
-        _check(_fn("core", "mv_attention_kv4")(*where, out.data_ptr() + row, dt, part_o, part_ml, tickets, N, nh, nkv, hd, scale, window, splits, gt,
-                                               head_tiles, _stream()), "mv_attention_kv4")
+    _guard("core", "kv4_cache", q.device, n_pages=pool.shape[0])
+    _check(_fn("core", "mv_attention_kv4")(*where, out.data_ptr() + row, dt, part_o, part_ml, tickets, N, nh, nkv, hd, scale, window, splits, gt,
+                                           head_tiles, _stream()), "mv_attention_kv4")
 
 
 def _attention_kv4_pages(q, pool, page_table, page_size, positions, seq_of, starts, out, nh, nkv, hd, scale, window, ws, cu, b0, b1, n0, n1, pages,

@@ -140,6 +140,7 @@ def test_read_refuses(over, match):
 @pytest.mark.parametrize("over,match", [
     (dict(hd=20), "multiple of 8"), (dict(nh=3), "not a multiple"), (dict(nh=0), "not a multiple"), (dict(out=torch.zeros(3, 64).bfloat16()), "agree"),
     (dict(host_lens=[4]), "3 rows"), (dict(host_lens=[3, 0], host_starts=[0, 0]), "a token or more"), (dict(host_starts=[0, 1]), "2 starts"),
+    (dict(scale=0.0), "positive"), (dict(scale=-0.1), "positive"), (dict(scale=float("nan")), "positive"), (dict(splits=0), "key splits"),
     (dict(), "CUDA devices only")])
 def test_attention_refuses(over, match):
     a = dict(q=torch.zeros(3, 64), pool=torch.zeros(5, 2, 4 * 24, dtype=torch.uint8), page_table=ints([[1, 2]]), positions=ints([0, 1, 2]),
