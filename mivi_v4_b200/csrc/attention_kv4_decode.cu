@@ -41,7 +41,9 @@ MV_GUARD_SETTER(attention_kv4_decode)
 
 namespace {
 
-constexpr int KD_WARPS = 4, KD_KEYS = 64;
+// A piece has a tile for every warp at least; up to KD_WHOLE tiles of keys are not cut: a second tile a warp costs less than the meeting of two
+// blocks (300 rows of one sequence: 5.0 us whole, 6.6 us in two; 1,000 rows behind a window: 10.8 us in pieces of 8, 9.6 us in pieces of 4).
+constexpr int KD_WARPS = 4, KD_KEYS = 64, KD_WHOLE = 8;
 
 __device__ __forceinline__ void bulk_load(unsigned dst, const void* src, unsigned bytes, unsigned bar) {
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
@@ -87,7 +89,7 @@ struct KdShape {
 
 // EXACT: HDP is the head size.  A column is token c / heads and head h0 + c % heads of the kv head's group, heads = min(group, 4 NT).  Only a token
 // whose place in its sequence's run is a multiple of tokens_per_tile begins a tile.  Block b works on kv head and head tile b % pairs of
-// piece b / pairs, counted over the tiles of columns.  piece: tiles of 64 keys in one, 0: such that there are ``blocks`` of them.
+// piece b / pairs, counted over the tiles of columns.  piece: tiles of 64 keys in one; 0: such that there are ``blocks`` of them.
 template <int HDP, bool EXACT, int NT>
 __global__ void __launch_bounds__(KD_WARPS * 32, KdShape<HDP, NT>::RESIDENT)
 attention_kv4_decode_kernel(const __nv_bfloat16* __restrict__ q, const unsigned char* __restrict__ pool, const int* __restrict__ page_table,
@@ -99,26 +101,24 @@ attention_kv4_decode_kernel(const __nv_bfloat16* __restrict__ q, const unsigned 
     using Shape = KdShape<HDP, NT>;
     constexpr int STAGES = Shape::STAGES, COLS = 4 * NT, MT = HDP / 16, W = HDP / 32;      // W: words of a lane's quarter of a row
     extern __shared__ __align__(128) unsigned char smem[];
-    __shared__ int scan[KD_WARPS], found[3], is_last;
+    __shared__ int scan[KD_WARPS], found[6], is_last;
     const int hd = EXACT ? HDP : hd_;
     const int warp = warp_index(), lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int pairs = nkv * head_tiles;
 
     // ---- which tile of columns, which piece of its keys
-    // tokens that the tile of columns that begins with row r holds (0: none begins there), and its tiles of keys
-    auto tokens_at = [&](int r) {
-        if (tokens_per_tile == 1) return 1;
-        const int b = seq_of[r];
-        if ((positions[r] - starts[b]) % tokens_per_tile) return 0;
-        int k = 1;
-        while (k < tokens_per_tile && r + k < N && seq_of[r + k] == b) ++k;
-        return k;
-    };
+    // of row r: its sequence and position, the tokens of the tile of columns that begins with it (0: none does) and their tiles of keys
+    int row_seq, row_pos, row_tokens;
     auto tiles_at = [&](int r) {
-        const int k = r < N ? tokens_at(r) : 0;
-        if (k == 0) return 0;
-        const int p = positions[r];
-        return (p + k - 1) / KD_KEYS + 1 - (window > 0 ? max(0, p - window + 1) / KD_KEYS : 0);
+        if (r >= N) return 0;
+        row_seq = seq_of[r];
+        row_pos = positions[r];
+        row_tokens = 1;
+        if (tokens_per_tile > 1) {
+            if ((row_pos - starts[row_seq]) % tokens_per_tile) return 0;
+            while (row_tokens < tokens_per_tile && r + row_tokens < N && seq_of[r + row_tokens] == row_seq) ++row_tokens;
+        }
+        return (row_pos + row_tokens - 1) / KD_KEYS + 1 - (window > 0 ? max(0, row_pos - window + 1) / KD_KEYS : 0);
     };
     auto block_sum = [&](int v, int& before) {                   // of one number a thread; before: of the threads before this one
         int inc = v;
@@ -139,12 +139,16 @@ attention_kv4_decode_kernel(const __nv_bfloat16* __restrict__ q, const unsigned 
         before = base + inc - v;
         return all;
     };
-    int n, part, parts;
+    int n, part, parts, seq, pos0, tokens;
     {
         int before, mine = tiles_at(threadIdx.x);                // (of the first 128 rows; usually all there are)
-        if (piece == 0) {
+        const bool given = piece > 0;
+        if (!given) {
             long long all = block_sum(mine, before);
-            for (int r0 = KD_WARPS * 32; r0 < N; r0 += KD_WARPS * 32) all += block_sum(tiles_at(r0 + threadIdx.x), before);
+            if (N > KD_WARPS * 32) {
+                for (int r0 = KD_WARPS * 32; r0 < N; r0 += KD_WARPS * 32) all += block_sum(tiles_at(r0 + threadIdx.x), before);
+                mine = tiles_at(threadIdx.x);
+            }
             // (half a piece a tile of columns is lost where its keys end: as many blocks are left to it)
             const int aim = max(blocks / 2, blocks - (N * pairs + 1) / 2);
             piece = max(KD_WARPS, (int)((all * pairs + aim - 1) / aim));
@@ -154,12 +158,15 @@ attention_kv4_decode_kernel(const __nv_bfloat16* __restrict__ q, const unsigned 
         int base = 0;
         for (int r0 = 0; r0 < N && base <= want; r0 += KD_WARPS * 32) {
             if (r0) mine = tiles_at(r0 + threadIdx.x);
-            const int count = (mine + piece - 1) / piece;
+            const int count = mine <= KD_WHOLE && !given ? (int)(mine > 0) : (mine + piece - 1) / piece;
             const int all = block_sum(count, before);
             if (want >= base + before && want < base + before + count) {
                 found[0] = r0 + threadIdx.x;
                 found[1] = want - base - before;
                 found[2] = count;
+                found[3] = row_seq;
+                found[4] = row_pos;
+                found[5] = row_tokens;
             }
             base += all;
         }
@@ -167,11 +174,13 @@ attention_kv4_decode_kernel(const __nv_bfloat16* __restrict__ q, const unsigned 
         n = found[0];
         part = found[1];
         parts = found[2];
+        seq = found[3];
+        pos0 = found[4];
+        tokens = found[5];
     }
     if (n < 0) return;
     const int pair = blockIdx.x % pairs, kvh = pair / head_tiles, h0 = (pair - kvh * head_tiles) * heads;
     const int group = nh / nkv, live_heads = min(heads, group - h0);
-    const int seq = seq_of[n], pos0 = positions[n], tokens = tokens_at(n);
     const int pos_last = pos0 + tokens - 1, lo_key = window > 0 ? max(0, pos0 - window + 1) : 0;
     const int* table = page_table + (size_t)seq * table_stride;
     const int page_size = 1 << page_shift;
@@ -190,7 +199,7 @@ attention_kv4_decode_kernel(const __nv_bfloat16* __restrict__ q, const unsigned 
 
     // this warp's tiles: every KD_WARPS-th of the piece's
     const int tile0 = lo_key / KD_KEYS, n_tiles = pos_last / KD_KEYS + 1 - tile0;
-    const int first = tile0 + part * piece + warp, past = tile0 + min(n_tiles, (part + 1) * piece);
+    const int first = tile0 + part * piece + warp, past = tile0 + (parts == 1 ? n_tiles : min(n_tiles, (part + 1) * piece));
     const int mine = first < past ? (past - first + KD_WARPS - 1) / KD_WARPS : 0;
     // where the first page of a tile lies: asked for a tile early, so that the copy need not wait for the page table
     auto page_of = [&](int i) { return i < mine ? mv_read_page(table[(first + i * KD_WARPS) * KD_KEYS >> page_shift]) : 0; };
@@ -233,45 +242,51 @@ attention_kv4_decode_kernel(const __nv_bfloat16* __restrict__ q, const unsigned 
         const int c = 4 * nt + (g >> 1), tok = c / heads, h = c - tok * heads;
         const bool live = tok < tokens && h < live_heads;
         const __nv_bfloat16* row = q + ((size_t)(n + (live ? tok : 0)) * nh + kvh * group + h0 + (live ? h : 0)) * hd;
-        float x[HDP / 4], top = 0.f;
-        bool fine = true;
+        uint4 raw[HDP / 32];                                     // two bfloat16 a word
+        __nv_bfloat162 big = __floats2bfloat162_rn(0.f, 0.f);
 #pragma unroll
         for (int w = 0; w < W; ++w) {
             const int d = t * (HDP / 4) + 8 * w;
-            if (live && (EXACT || d < hd)) mv_load8(row + d, x + 8 * w);
-            else
+            raw[w] = live && (EXACT || d < hd) ? *reinterpret_cast<const uint4*>(row + d) : make_uint4(0u, 0u, 0u, 0u);
+            const unsigned x[4] = {raw[w].x, raw[w].y, raw[w].z, raw[w].w};
 #pragma unroll
-                for (int e = 0; e < 8; ++e) x[8 * w + e] = 0.f;
+            for (int e = 0; e < 4; ++e) big = __hmax2_nan(big, __habs2(*reinterpret_cast<const __nv_bfloat162*>(&x[e])));
         }
-#pragma unroll
-        for (int e = 0; e < HDP / 4; ++e) {
-            top = fmaxf(top, fabsf(x[e]));
-            fine = fine && fabsf(x[e]) < INFINITY;
-        }
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        const unsigned quad = 0xfu << (lane & ~3);
-        fine = (__ballot_sync(0xffffffffu, fine) & quad) == quad;
+        // (not a number, where one of the elements is none: the row's scores are none then)
+        float top = __bfloat162float(__hmax_nan(__low2bfloat16(big), __high2bfloat16(big)));
+        const float t1 = __shfl_xor_sync(0xffffffffu, top, 1);
+        top = top > t1 || top != top ? top : t1;
+        const float t2 = __shfl_xor_sync(0xffffffffu, top, 2);
+        top = top > t2 || top != top ? top : t2;
+        const bool fine = top < INFINITY;
         // the largest element times 2^up: at least 2^13, and at most 127 * 256, so that its pieces are bytes
         int up = top > 0.f && fine ? 14 - ((int)(__float_as_uint(top) >> 23) - 127) : 0;
-        if (top * pow2f(up >> 1) * pow2f(up - (up >> 1)) > 32512.f) --up;
-        const float up0 = pow2f(up >> 1), up1 = pow2f(up - (up >> 1));
-        int sum = 0;
+        float up0 = pow2f(up >> 1), up1 = pow2f(up - (up >> 1));
+        if (top * up0 * up1 > 32512.f) { --up; up1 *= 0.5f; }
+        if (!fine) up0 = 0.f;
+        // Added to 1.5 * 2^23 a number from -2^22 to 2^22 is rounded to a whole one, which stands in the low bits.  Its low piece, from -128 to
+        // 127, is its lowest byte; its high piece the next one, once 128 is added.
+        const unsigned piece_of = g & 1 ? 0x6240u : 0x7351u, round = g & 1 ? 0u : 128u;
+        unsigned sum = 0u;
 #pragma unroll
         for (int w = 0; w < W; ++w) {
+            const unsigned x[4] = {raw[w].x, raw[w].y, raw[w].z, raw[w].w};
 #pragma unroll
             for (int odd = 0; odd < 2; ++odd) {
-                unsigned bytes = 0u;
+                unsigned v[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const int v = fine ? __float2int_rn(x[8 * w + 2 * e + odd] * up0 * up1) : 0;
-                    const int low = ((v + 128) & 255) - 128;
-                    sum += v;
-                    bytes |= (unsigned)((g & 1 ? low : (v - low) >> 8) & 255) << (8 * e);
+                    const float f = __uint_as_float(odd ? x[e] & 0xffff0000u : x[e] << 16);
+                    v[e] = __float_as_uint(fmaf(f * up0, up1, 12582912.f));
+                    sum += v[e];
+                    v[e] += round;
                 }
-                qf[nt][w][odd] = bytes;
+                // bytes 0 (or 1) of v[0], v[1] and of v[2], v[3], then one of each after the other
+                const unsigned lo = __byte_perm(v[0], v[1], piece_of), hi = __byte_perm(v[2], v[3], piece_of);
+                qf[nt][w][odd] = __byte_perm(lo, hi, 0x5410);
             }
         }
+        sum -= (unsigned)(HDP / 4) * 0x4b400000u;
         sum += __shfl_xor_sync(0xffffffffu, sum, 1);
         sum += __shfl_xor_sync(0xffffffffu, sum, 2);
         // A score is (q . code) step + sum(q) zero, below 2^25 times a row's numbers: for queries below 2^34 it is taken times 2^-30, so
@@ -279,7 +294,7 @@ attention_kv4_decode_kernel(const __nv_bfloat16* __restrict__ q, const unsigned 
         const int spare = up > -20 ? -30 : 0;
         const int ex = -up - spare;
         const float f = fine ? scale_log2 * pow2f(max(-126, min(127, ex))) : NAN;
-        const float sm = (float)sum * pow2f(spare);
+        const float sm = (float)(int)sum * pow2f(spare);
         const int at = live ? pos0 + tok : -1;
         // lane t scores column 4 nt + t, whose pieces lie in the lanes of g = 2t and 2t + 1
         lsc[nt] = __shfl_sync(0xffffffffu, f, 8 * t);
@@ -544,13 +559,15 @@ attention_kv4_decode_kernel(const __nv_bfloat16* __restrict__ q, const unsigned 
         }
     }
     if (parts == 1) return;
-    __threadfence();
     __syncthreads();
     int* ticket = tickets + (size_t)n * pairs + pair;
-    if (threadIdx.x == 0) is_last = atomicAdd(ticket, 1) == parts - 1;
+    if (threadIdx.x == 0) {
+        __threadfence();                                         // (the barrier before it makes it stand for the whole block)
+        is_last = atomicAdd(ticket, 1) == parts - 1;
+        __threadfence();
+    }
     __syncthreads();
     if (!is_last) return;
-    __threadfence();
     for (int e = threadIdx.x; e < used * (hd >> 2); e += KD_WARPS * 32) {
         const int c0 = e / (hd >> 2), d = (e - c0 * (hd >> 2)) * 4;
         const int tok = c0 / live_heads, h = c0 - tok * live_heads;

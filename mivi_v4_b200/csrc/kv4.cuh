@@ -29,11 +29,15 @@ __device__ __forceinline__ void kv4_poison(Kv4Params& p) {
     if (!(fabsf(p.vs) < INFINITY)) { p.ks = NAN; p.vs = 0.f; p.vz = 0.f; }
 }
 
-// The step of a row with these extremes, zero being bf16(lo).  Halves: hi - lo may pass the largest float; and where zero + 15 steps would,
-// the step is the next lower one.
-__device__ __forceinline__ float kv4_step(float hi, float zero) {
-    const float step = __bfloat162float(__float2bfloat16_rn(fmaxf(0.5f * hi - 0.5f * zero, 0.f) / 7.5f));
+// A step as bfloat16: the next lower one where zero + 15 steps would pass the largest float.
+__device__ __forceinline__ float kv4_round_step(float exact, float zero) {
+    const float step = __bfloat162float(__float2bfloat16_rn(exact));
     return fmaf(15.f, step, zero) == INFINITY ? __uint_as_float(__float_as_uint(step) - 0x10000u) : step;
+}
+// The step of a row whose largest element is hi, zero being bf16 of its smallest: (hi - zero) times 1 / 15, in 32 bits.  (Halves: the difference
+// may pass the largest float.)
+__device__ __forceinline__ float kv4_step(float hi, float zero) {
+    return kv4_round_step(2.f * (fmaxf(0.5f * hi - 0.5f * zero, 0.f) * (1.f / 15.f)), zero);
 }
 __device__ __forceinline__ unsigned kv4_code(float x, float zero, float step) {
     if (step <= 0.f) return 0u;

@@ -8,132 +8,333 @@
 MV_GUARD_SETTER(kv4_cache)
 
 // ------------------------------------------------- q/k norm, rotation, quantised append
-// One warp per token and head: nh query heads, then nkv key heads, then nkv value heads, as they lie in a row of the fused projection.
-// A lane holds the neighbouring elements 2i and 2i + 1 with i = lane, lane + 32, ...: one byte of codes.
-__global__ void __launch_bounds__(256)
+// Block = one token: nh query heads, then nkv key heads, then nkv value heads, as they lie in a row of the fused projection.  A head's row
+// lies in LPH lanes, four neighbouring elements each (CH times), so a warp takes 32 / LPH heads of a kind a round; its rows are asked for
+// before the token's angles are worked out.  The projection's rows, 4 bytes an element, are what cannot be avoided; the rest is
+// instructions, kept few: angles once a block, weights and turns of a lane's elements once a warp, quotients as products (below).
+//
+// Keys are worked out in 64 bits, from the sum of squares to the code: a code is a decision, and 32 bits move one in a million of them to the
+// other side of its border (by a step, 0.3 of the row's mean square).  A key then stands in the cache as the formulas say, whatever the
+// order of a sum.  The angle takes 64 bits anyway: a product of 32 bits is off by 2^-25 of it, a thousandth at position 32,768.  Queries,
+// which are rounded to the model's dtype and decide nothing, take 32 bits from there; values are used as they come.
+constexpr int KP_ROUNDS = 4;
+
+// Sine and cosine of the angle a in 64 bits: a less the nearest multiple of a quarter turn, then their series.  Within pi / 4 the first terms left
+// out are x^17 / 17! and x^18 / 18!, below 2^-54.  (Off by 2^-52 of a on top, that is by the quarter turn's own last place times their
+// number.)
+__device__ __forceinline__ double2 kv4_turn(double a) {
+    const double k = rint(a * 0.6366197723675814);               // 2 / pi
+    const double x = fma(k, -1.5707963267948966, a), z = x * x;
+    double s = -1.0 / 1307674368000.0, c = 1.0 / 20922789888000.0;
+    s = fma(s, z, 1.0 / 6227020800.0);
+    c = fma(c, z, -1.0 / 87178291200.0);
+    s = fma(s, z, -1.0 / 39916800.0);
+    c = fma(c, z, 1.0 / 479001600.0);
+    s = fma(s, z, 1.0 / 362880.0);
+    c = fma(c, z, -1.0 / 3628800.0);
+    s = fma(s, z, -1.0 / 5040.0);
+    c = fma(c, z, 1.0 / 40320.0);
+    s = fma(s, z, 1.0 / 120.0);
+    c = fma(c, z, -1.0 / 720.0);
+    s = fma(s, z, -1.0 / 6.0);
+    c = fma(c, z, 1.0 / 24.0);
+    s = fma(s * z, x, x);
+    c = fma(fma(c, z, -0.5), z, 1.0);
+    const int quarter = (int)((long long)k & 3);
+    const double cc = quarter & 1 ? s : c, ss = quarter & 1 ? c : s;
+    return make_double2(quarter == 1 || quarter == 2 ? -cc : cc, quarter & 2 ? -ss : ss);
+}
+// 1 / sqrt(x) and 1 / x in 64 bits by Newton's steps from 32-bit ones (each doubles the places); x in the normal range of 32 bits, or the
+// 32-bit value is kept (0, infinity, not a number).
+__device__ __forceinline__ double kv4_rsqrt(double x) {
+    const float f = rsqrtf((float)x);
+    double r = (double)f;
+    if (!(f > 1e-18f && f < 1e18f)) return r;
+    r = r * fma(-0.5 * x * r, r, 1.5);
+    return r * fma(-0.5 * x * r, r, 1.5);
+}
+__device__ __forceinline__ double kv4_inverse(float x) {
+    double r = (double)(1.0f / x);
+    if (!(x > 1e-37f && x < 1e37f)) return 1.0 / (double)x;
+    return r * fma(-(double)x, r, 2.0);
+}
+
+template <int LPH, int CH, typename T>
+__global__ void __launch_bounds__(256, CH == 1 ? 4 : 2)
 kv4_prepare_kernel(const float* __restrict__ qkv, const float* __restrict__ wq, const float* __restrict__ wk, float eps,
                    const float* __restrict__ inv_freq, int half_split, const int* __restrict__ positions,
                    const int* __restrict__ seq_of, const int* __restrict__ page_table, int table_stride, int page_shift,
-                   unsigned char* __restrict__ pool, void* __restrict__ q_out, int q_dtype, int N, int nh, int nkv, int hd) {
+                   unsigned char* __restrict__ pool, T* __restrict__ q_out, int nh, int nkv, int hd, double per_hd) {
     mv_pdl_begin();
-    const long long wid = ((long long)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
-    const int lane = threadIdx.x & 31, slots = nh + 2 * nkv;
-    if (wid >= (long long)N * slots) return;
-    const int n = (int)(wid / slots), hs = (int)(wid - (long long)n * slots);
-    const bool is_q = hs < nh, is_k = !is_q && hs < nh + nkv;
-    const int half = hd >> 1;
-    constexpr int MAXJ = KV4_MAX_HEAD_DIM / 64;
-    const float* row = qkv + (size_t)wid * hd;
+    __shared__ double2 turn[KV4_MAX_HEAD_DIM / 2];               // cosine and sine of the token's angles
+    __shared__ float2 turn32[KV4_MAX_HEAD_DIM / 2];
+    constexpr int HPW = 32 / LPH;
+    const int n = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = lane & (LPH - 1), hsel = lane / LPH;
+    const int warps = blockDim.x >> 5, slots = nh + 2 * nkv, half = hd >> 1, chunks = hd >> 2, shift = half >> 2;
+    // rounds of one kind of head each; a warp's first: of queries its own number, of keys too, of values the next free warps'
+    const int rq = (nh + HPW - 1) / HPW, rk = (nkv + HPW - 1) / HPW;
+    const int first_v = (warp + warps - rk % warps) % warps;
+    const float4 none = make_float4(0.f, 0.f, 0.f, 0.f);
+    const float* rows = qkv + (size_t)n * slots * hd;
+    auto load = [&](float4 (&to)[CH], int slot0, int h, int count) {        // head h of ``count`` that begin at slot0
+#pragma unroll
+        for (int c = 0; c < CH; ++c)
+            to[c] = h < count && sub + LPH * c < chunks ? *reinterpret_cast<const float4*>(rows + (size_t)(slot0 + h) * hd + 4 * (sub + LPH * c)) : none;
+    };
+    float4 qx[KP_ROUNDS][CH], kx[CH], vx[CH];
+#pragma unroll
+    for (int u = 0; u < KP_ROUNDS; ++u) load(qx[u], 0, (warp + u * warps) * HPW + hsel, nh);
+    load(kx, nh, warp * HPW + hsel, nkv);
+    load(vx, nh + nkv, first_v * HPW + hsel, nkv);
     const int pos = positions[n];
-    float2 x[MAXJ];
-#pragma unroll
-    for (int j = 0; j < MAXJ; ++j) {
-        const int i = lane + 32 * j;
-        x[j] = i < half ? *reinterpret_cast<const float2*>(row + 2 * i) : make_float2(0.f, 0.f);
-    }
-    if (is_q || is_k) {
-        const float* w = is_q ? wq : wk;
-        float scale = 1.f;
-        if (w) {
-            float ss = 0.f;
-#pragma unroll
-            for (int j = 0; j < MAXJ; ++j) ss = fmaf(x[j].x, x[j].x, fmaf(x[j].y, x[j].y, ss));
-            ss = mv_warp_sum(ss);
-            scale = 1.0f / sqrtf(ss / (float)hd + eps);
-        }
-        // The angle is worked out in 64 bits and brought into one turn: a product of 32 bits is off by 2^-25 of the angle, which at
-        // position 32,768 is a thousandth of a turn's radian, more than enough to move a code.
-        auto turn = [&](int i, float& c, float& s) {
-            const double a = (double)pos * (double)inv_freq[i];
-            const double r = fma(rint(a * 0.15915494309189535), -6.283185307179586, a);
-            sincosf((float)r, &s, &c);
-        };
-#pragma unroll
-        for (int j = 0; j < MAXJ; ++j) {
-            const int i = lane + 32 * j;
-            if (i >= half) break;
-            float2 y = x[j];
-            if (w) {
-                const float2 ww = *reinterpret_cast<const float2*>(w + 2 * i);
-                y.x = y.x * scale * ww.x;
-                y.y = y.y * scale * ww.y;
-            }
-            if (inv_freq && !half_split) {                       // pairs (2i, 2i + 1)
-                float c, s;
-                turn(i, c, s);
-                y = make_float2(y.x * c - y.y * s, y.x * s + y.y * c);
-            } else if (inv_freq) {                               // pairs (i, i + half): the partners are the neighbours 2i -+ half
-                const int e = 2 * i, lo = e < half ? e : e - half;
-                const int other = e < half ? e + half : e - half;
-                float2 z = *reinterpret_cast<const float2*>(row + other);
-                if (w) {
-                    const float2 ww = *reinterpret_cast<const float2*>(w + other);
-                    z.x = z.x * scale * ww.x;
-                    z.y = z.y * scale * ww.y;
-                }
-                float c0, s0, c1, s1;
-                turn(lo, c0, s0);
-                turn(lo + 1, c1, s1);
-                y = e < half ? make_float2(y.x * c0 - z.x * s0, y.y * c1 - z.y * s1) : make_float2(z.x * s0 + y.x * c0, z.y * s1 + y.y * c1);
-            }
-            x[j] = y;
-        }
-    }
-    if (is_q) {
-#pragma unroll
-        for (int j = 0; j < MAXJ; ++j) {
-            const int i = lane + 32 * j;
-            if (i >= half) break;
-            const size_t at = ((size_t)n * nh + hs) * hd + 2 * i;
-            if (q_dtype == MV_DT_BF16) mv_store2((__nv_bfloat16*)q_out + at, x[j].x, x[j].y);
-            else mv_store2((float*)q_out + at, x[j].x, x[j].y);
-        }
-        return;
-    }
-    float lo = INFINITY, hi = -INFINITY;
-    bool fine = true;
-#pragma unroll
-    for (int j = 0; j < MAXJ; ++j) {
-        if (lane + 32 * j >= half) break;
-        lo = fminf(lo, fminf(x[j].x, x[j].y));
-        hi = fmaxf(hi, fmaxf(x[j].x, x[j].y));
-        fine = fine && fabsf(x[j].x) < INFINITY && fabsf(x[j].y) < INFINITY;
-    }
-    lo = -mv_warp_max(-lo);
-    hi = mv_warp_max(hi);
-    fine = __all_sync(0xffffffffu, fine);
-    float zero = __bfloat162float(__float2bfloat16_rn(lo));
-    // (the lowest floats would round to -infinity)
-    zero = fminf(fmaxf(zero, -3.3895313892515355e38f), 3.3895313892515355e38f);
-    float step = kv4_step(hi, zero);
-    if (!fine) { zero = NAN; step = NAN; }
     const int page = page_table[(size_t)seq_of[n] * table_stride + (pos >> page_shift)];
-    if (!mv_page_ok(page)) return;
+    if (inv_freq)
+        for (int i = threadIdx.x; i < half; i += blockDim.x) {
+            const double2 d = kv4_turn((double)pos * (double)inv_freq[i]);
+            turn[i] = d;
+            turn32[i] = make_float2((float)d.x, (float)d.y);
+        }
+    __syncthreads();
     const int page_size = 1 << page_shift, at = pos & (page_size - 1);
-    const int g = is_k ? hs - nh : hs - nh - nkv;
-    unsigned char* base = pool + ((size_t)page * nkv + g) * kv4_head_bytes(page_size, hd);
-    unsigned char* codes = base + ((size_t)(is_k ? 0 : page_size) + at) * half;
+    const bool writes = mv_page_ok(page);
+    unsigned char* const where = pool + (size_t)(writes ? page : 0) * nkv * kv4_head_bytes(page_size, hd);
+    // which angle an element turns by, and whether it is its pair's first: pairs (2i, 2i + 1), or (i, i + half) with the other one in
+    // the chunk ``shift`` on or back
+    auto angle_of = [&](int c, int e) {
+        const int i = min(sub + LPH * c, chunks - 1);
+        return half_split ? 4 * (i < shift ? i : i - shift) + e : 2 * i + (e >> 1);
+    };
+    auto partner = [&](auto here, auto there, int c) {           // element of the pair's other chunk: in array 0 or array CH - 1
+        const int i = sub + LPH * c, j = i < shift ? i + shift : i - shift, from = (lane & ~(LPH - 1)) | (j & (LPH - 1));
+        const auto a = __shfl_sync(0xffffffffu, here, from);
+        const auto b = CH == 2 ? __shfl_sync(0xffffffffu, there, from) : a;
+        return CH == 2 && j / LPH != 0 ? b : a;
+    };
+    auto rotate = [&](auto (&y)[CH][4], const auto (&cs)[CH][4], const auto (&sn)[CH][4]) {
+        if (!half_split) {
 #pragma unroll
-    for (int j = 0; j < MAXJ; ++j) {
-        const int i = lane + 32 * j;
-        if (i >= half) break;
-        codes[i] = fine ? (unsigned char)(kv4_code(x[j].x, zero, step) | kv4_code(x[j].y, zero, step) << 4) : 0;
+            for (int c = 0; c < CH; ++c)
+#pragma unroll
+                for (int e = 0; e < 4; e += 2) {
+                    const auto a = y[c][e], b = y[c][e + 1];
+                    y[c][e] = a * cs[c][e] - b * sn[c][e];
+                    y[c][e + 1] = a * sn[c][e] + b * cs[c][e];
+                }
+        } else {
+            auto z = y[0][0];
+            decltype(z) w[CH][4];
+#pragma unroll
+            for (int c = 0; c < CH; ++c)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) w[c][e] = partner(y[0][e], y[CH - 1][e], c);
+#pragma unroll
+            for (int c = 0; c < CH; ++c)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const auto s = sub + LPH * c < shift ? -sn[c][e] : sn[c][e];
+                    y[c][e] = w[c][e] * s + y[c][e] * cs[c][e];
+                }
+        }
+    };
+    {   // ---- queries
+        float w[CH][4], cs[CH][4], sn[CH][4];
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+            float4 f = make_float4(1.f, 1.f, 1.f, 1.f);
+            if (wq && sub + LPH * c < chunks) f = *reinterpret_cast<const float4*>(wq + 4 * (sub + LPH * c));
+            w[c][0] = f.x; w[c][1] = f.y; w[c][2] = f.z; w[c][3] = f.w;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float2 d = inv_freq ? turn32[angle_of(c, e)] : make_float2(1.f, 0.f);
+                cs[c][e] = d.x;
+                sn[c][e] = d.y;
+            }
+        }
+        for (int r0 = warp; r0 < rq; r0 += KP_ROUNDS * warps) {
+            if (r0 != warp)
+#pragma unroll
+                for (int u = 0; u < KP_ROUNDS; ++u) load(qx[u], 0, (r0 + u * warps) * HPW + hsel, nh);
+#pragma unroll
+            for (int u = 0; u < KP_ROUNDS; ++u) {
+                const int h = (r0 + u * warps) * HPW + hsel;
+                if (r0 + u * warps >= rq) break;
+                float y[CH][4];
+#pragma unroll
+                for (int c = 0; c < CH; ++c) { y[c][0] = qx[u][c].x; y[c][1] = qx[u][c].y; y[c][2] = qx[u][c].z; y[c][3] = qx[u][c].w; }
+                if (wq) {
+                    float ss = 0.f;
+#pragma unroll
+                    for (int c = 0; c < CH; ++c)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) ss = fmaf(y[c][e], y[c][e], ss);
+#pragma unroll
+                    for (int o = LPH >> 1; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+                    const float m = fmaf(ss, (float)per_hd, eps);
+                    float scale = rsqrtf(m);
+                    if (scale > 1e-18f && scale < 1e18f) scale = scale * fmaf(-0.5f * m * scale, scale, 1.5f);
+#pragma unroll
+                    for (int c = 0; c < CH; ++c)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) y[c][e] = y[c][e] * scale * w[c][e];
+                }
+                if (inv_freq) rotate(y, cs, sn);
+#pragma unroll
+                for (int c = 0; c < CH; ++c)
+                    if (h < nh && sub + LPH * c < chunks)
+                        mv_store4(q_out + ((size_t)n * nh + h) * hd + 4 * (sub + LPH * c), y[c][0], y[c][1], y[c][2], y[c][3]);
+            }
+        }
     }
-    if (lane == 0)
-        *reinterpret_cast<unsigned*>(base + (size_t)page_size * hd + (size_t)at * 8 + (is_k ? 0 : 4)) = kv4_pack_params(step, zero);
+    // ---- a row's ends (rounding keeps the order, so a key's may be looked for in 32 bits), its zero and step, and its way to the pool
+    auto hold = [&](const float (&x)[CH][4], int kv, int g, auto step_of, auto code_of) {
+        float lo = INFINITY, hi = -INFINITY;
+        bool fine = true;
+#pragma unroll
+        for (int c = 0; c < CH; ++c)
+            if (sub + LPH * c < chunks)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    lo = fminf(lo, x[c][e]);
+                    hi = fmaxf(hi, x[c][e]);
+                    fine = fine && fabsf(x[c][e]) < INFINITY;
+                }
+#pragma unroll
+        for (int o = LPH >> 1; o > 0; o >>= 1) {
+            lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+            hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+        }
+        const unsigned group = LPH == 32 ? 0xffffffffu : ((1u << (LPH & 31)) - 1u) << (lane & ~(LPH - 1));
+        fine = (__ballot_sync(0xffffffffu, fine) & group) == group;
+        // (the lowest floats would round to -infinity)
+        float zero = fminf(fmaxf(__bfloat162float(__float2bfloat16_rn(lo)), -3.3895313892515355e38f), 3.3895313892515355e38f);
+        float step = step_of(hi, zero);
+        unsigned code[CH];
+#pragma unroll
+        for (int c = 0; c < CH; ++c) code[c] = 0u;
+        if (step > 0.f && fine) code_of(code, zero, step);
+        if (!fine) zero = step = NAN;
+        if (g < nkv && writes) {
+            unsigned char* base = where + (size_t)g * kv4_head_bytes(page_size, hd);
+            unsigned char* codes = base + ((size_t)(kv ? page_size : 0) + at) * half;
+#pragma unroll
+            for (int c = 0; c < CH; ++c)
+                if (sub + LPH * c < chunks) *reinterpret_cast<unsigned short*>(codes + 2 * (sub + LPH * c)) = (unsigned short)code[c];
+            if (sub == 0)
+                *reinterpret_cast<unsigned*>(base + (size_t)page_size * hd + (size_t)at * 8 + 4 * kv) = kv4_pack_params(step, zero);
+        }
+    };
+    // ---- keys, in 64 bits
+    for (int r = warp; r < rk; r += warps) {
+        if (r != warp) load(kx, nh, r * HPW + hsel, nkv);
+        double y[CH][4];
+#pragma unroll
+        for (int c = 0; c < CH; ++c) { y[c][0] = kx[c].x; y[c][1] = kx[c].y; y[c][2] = kx[c].z; y[c][3] = kx[c].w; }
+        if (wk) {
+            double ss = 0.0;
+#pragma unroll
+            for (int c = 0; c < CH; ++c)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) ss = fma(y[c][e], y[c][e], ss);
+#pragma unroll
+            for (int o = LPH >> 1; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+            const double scale = kv4_rsqrt(fma(ss, per_hd, (double)eps));
+#pragma unroll
+            for (int c = 0; c < CH; ++c) {
+                float4 f = none;
+                if (sub + LPH * c < chunks) f = *reinterpret_cast<const float4*>(wk + 4 * (sub + LPH * c));
+                y[c][0] *= scale * f.x; y[c][1] *= scale * f.y; y[c][2] *= scale * f.z; y[c][3] *= scale * f.w;
+            }
+        }
+        if (inv_freq) {
+            double cs[CH][4], sn[CH][4];
+#pragma unroll
+            for (int c = 0; c < CH; ++c)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const double2 d = turn[angle_of(c, e)];
+                    cs[c][e] = d.x;
+                    sn[c][e] = d.y;
+                }
+            rotate(y, cs, sn);
+        }
+        float x[CH][4];
+#pragma unroll
+        for (int c = 0; c < CH; ++c)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[c][e] = (float)y[c][e];
+        hold(x, 0, r * HPW + hsel, [&](float hi, float zero) {
+            // the largest element in 64 bits, among those that are it in 32
+            double top = -INFINITY;
+#pragma unroll
+            for (int c = 0; c < CH; ++c)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (x[c][e] == hi && y[c][e] > top && sub + LPH * c < chunks) top = y[c][e];
+#pragma unroll
+            for (int o = LPH >> 1; o > 0; o >>= 1) top = fmax(top, __shfl_xor_sync(0xffffffffu, top, o));
+            return kv4_round_step((float)(fmax(top - (double)zero, 0.0) * (1.0 / 15.0)), zero);
+        }, [&](unsigned (&code)[CH], float zero, float step) {
+            const double per_step = kv4_inverse(step), from = (double)zero;
+#pragma unroll
+            for (int c = 0; c < CH; ++c)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    // to the nearest whole number, ties to the even one: it stands in the low bits of a number of 1.5 * 2^52
+                    const double t = fma(y[c][e] - from, per_step, 6755399441055744.0);
+                    code[c] |= (unsigned)min(max(__double2loint(t), 0), 15) << (4 * e);
+                }
+        });
+    }
+    // ---- values.  A quotient (x - zero) / step, rounded to 32 bits and then to a whole number, is a product by 1 / step rounded once, unless it
+    // lies next to a border: then it is divided.
+    for (int r = first_v; r < rk; r += warps) {
+        if (r != first_v) load(vx, nh + nkv, r * HPW + hsel, nkv);
+        float x[CH][4];
+#pragma unroll
+        for (int c = 0; c < CH; ++c) { x[c][0] = vx[c].x; x[c][1] = vx[c].y; x[c][2] = vx[c].z; x[c][3] = vx[c].w; }
+        hold(x, 1, r * HPW + hsel, [](float hi, float zero) { return kv4_step(hi, zero); }, [&](unsigned (&code)[CH], float zero, float step) {
+            const float per_step = step > 1e-30f && step < 1e30f ? 2.0f / step : 0.f, from = -0.5f * zero;
+#pragma unroll
+            for (int c = 0; c < CH; ++c)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float t = fmaf(0.5f, x[c][e], from) * per_step, whole = rintf(t);
+                    unsigned v = (unsigned)fminf(fmaxf(whole, 0.f), 15.f);
+                    if (fabsf(t - whole) > 0.4999f || per_step == 0.f) v = kv4_code(x[c][e], zero, step);
+                    code[c] |= v << (4 * e);
+                }
+        });
+    }
 }
 
-// qkv float32 [N, (nh + 2 nkv) * hd]; pool [pages, nkv, page_size * (hd + 8)] bytes.  q_out [N, nh * hd] in q_dtype.
+// qkv float32 [N, (nh + 2 nkv) * hd]; pool [pages, nkv, page_size * (hd + 8)] bytes.  q_out [N, nh * hd] in q_dtype.  Everything on 16 bytes.
 MV_API int mv_kv4_prepare(const float* qkv, const float* wq, const float* wk, float eps, const float* inv_freq, int half_split,
                           const int* positions, const int* seq_of, const int* page_table, int table_stride, int page_size,
                           void* pool, void* q_out, int q_dtype, int N, int nh, int nkv, int hd, cudaStream_t stream) {
     if (N <= 0) return 0;
-    if (hd % 8 || hd > KV4_MAX_HEAD_DIM || page_size < 1 || (page_size & (page_size - 1)) || nkv < 1) return (int)cudaErrorInvalidValue;
+    if (hd % 8 || hd < 8 || hd > KV4_MAX_HEAD_DIM || page_size < 1 || (page_size & (page_size - 1)) || nkv < 1 ||
+        (((uintptr_t)qkv | (uintptr_t)wq | (uintptr_t)wk | (uintptr_t)q_out | (uintptr_t)pool) & 15))
+        return (int)cudaErrorInvalidValue;
     int page_shift = 0;
     while ((1 << page_shift) < page_size) ++page_shift;
-    const long long warps = (long long)N * (nh + 2 * nkv);
-    mv_launch(kv4_prepare_kernel, dim3((unsigned)((warps + 7) / 8)), 256, 0, stream, qkv, wq, wk, eps, inv_freq, half_split, positions,
-              seq_of, page_table, table_stride, page_shift, (unsigned char*)pool, q_out, q_dtype, N, nh, nkv, hd);
+    // Few tokens: a warp a round, for the least latency; many: four warps a token, which share its angles.
+    const int lph = hd <= 32 ? 8 : hd <= 64 ? 16 : 32, hpw = 32 / lph;
+    const int rounds = (nh + hpw - 1) / hpw + 2 * ((nkv + hpw - 1) / hpw);
+    const int warps = N >= 296 ? (rounds < 4 ? rounds : 4) : (rounds < 8 ? rounds : 8);
+#define MV_GO(LPH, CH, T)                                                                                                                  \
+    mv_launch(kv4_prepare_kernel<LPH, CH, T>, dim3(N), 32 * warps, 0, stream, qkv, wq, wk, eps, inv_freq, half_split, positions, seq_of,   \
+              page_table, table_stride, page_shift, (unsigned char*)pool, (T*)q_out, nh, nkv, hd, 1.0 / hd)
+#define MV_HD(T)                                                                                                                           \
+    do {                                                                                                                                   \
+        if (hd <= 32) MV_GO(8, 1, T);                                                                                                      \
+        else if (hd <= 64) MV_GO(16, 1, T);                                                                                                \
+        else if (hd <= 128) MV_GO(32, 1, T);                                                                                               \
+        else MV_GO(32, 2, T);                                                                                                              \
+    } while (0)
+    if (q_dtype == MV_DT_BF16) MV_HD(__nv_bfloat16);
+    else MV_HD(float);
+#undef MV_HD
+#undef MV_GO
     return mv_launch_status();
 }
 

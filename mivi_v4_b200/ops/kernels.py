@@ -2645,16 +2645,9 @@ def _check_kv4(pool: torch.Tensor, nkv: int, hd: int, what: str) -> int:
     return page_size
 
 
-def _need_all(what: str, specs) -> int:
-    """``_need`` for [(name, tensor, dtype, shape)] at once, all on one device, the current one; returns its number.  One look
-    at each tensor while all is well (a call's checks take as long as its launch); what is wrong is worded by ``_need``."""
-    dev = specs[0][1].get_device()
-    for name, t, dtype, shape in specs:
-        if t is not None and (t.get_device() != dev or t.dtype != dtype or t.shape != shape or not t.is_contiguous()):
-            break
-    else:
-        if dev >= 0 and (_raw_device is None or _raw_device() == dev):
-            return dev
+def _misfit(what: str, specs) -> None:
+    """Words what is wrong with one of [(name, tensor, dtype, shape)], which have to lie on one device, the current one.  The wrappers
+    below look at each tensor once (their checks take as long as the launch) and come here when something does not fit."""
     first = specs[0][1]
     for name, t, dtype, shape in specs:
         _need(t, name, dtype, shape, True)
@@ -2662,7 +2655,10 @@ def _need_all(what: str, specs) -> int:
             raise KernelError(f"{what}: {name} is on {t.device}, not on {first.device}")
     if first.device.index != torch.cuda.current_device():
         raise KernelError(f"{what}: the tensors are on {first.device} but the current device is cuda:{torch.cuda.current_device()}")
-    return first.device.index
+
+
+def _is_current(dev: int) -> bool:
+    return dev >= 0 and dev == (_raw_device() if _raw_device is not None else torch.cuda.current_device())
 
 
 def _table_shape(page_table: torch.Tensor, what: str):
@@ -2687,20 +2683,34 @@ def kv4_prepare(qkv: torch.Tensor, wq: Optional[torch.Tensor], wk: Optional[torc
     if nh < 1:
         raise KernelError(f"kv4_prepare: {nh} heads")
     table_shape = _table_shape(page_table, "kv4_prepare")
-    dt = _dt(q_out)
-    f32, i32 = torch.float32, torch.int32
-    _need_all("kv4_prepare", (("qkv", qkv, f32, (N, (nh + 2 * nkv) * hd)), ("q norm weight", wq, f32, (hd,)), ("k norm weight", wk, f32, (hd,)),
-                              ("inv_freq", inv_freq, f32, (hd // 2,)), ("positions", positions, i32, (N,)), ("seq_of", seq_of, i32, (N,)),
-                              ("page table", page_table, i32, table_shape), ("cache pool", pool, torch.uint8, pool.shape),
-                              ("q out", q_out, q_out.dtype, (N, nh * hd))))
+    dt, dev, f32, i32 = _dt(q_out), qkv.get_device(), torch.float32, torch.int32
+    wq_ptr = wk_ptr = freq_ptr = None
+    fits = (qkv.dtype is f32 and qkv.shape == (N, (nh + 2 * nkv) * hd) and qkv.is_contiguous() and _is_current(dev)
+            and q_out.get_device() == dev and q_out.shape == (N, nh * hd) and q_out.is_contiguous()
+            and pool.get_device() == dev and pool.is_contiguous()
+            and positions.get_device() == dev and positions.dtype is i32 and positions.shape == (N,) and positions.is_contiguous()
+            and seq_of.get_device() == dev and seq_of.dtype is i32 and seq_of.shape == (N,) and seq_of.is_contiguous()
+            and page_table.get_device() == dev and page_table.dtype is i32 and page_table.is_contiguous())
+    if fits and wq is not None:
+        fits = wq.get_device() == dev and wq.dtype is f32 and wq.shape == (hd,) and wq.is_contiguous()
+        wq_ptr = wq.data_ptr()
+    if fits and wk is not None:
+        fits = wk.get_device() == dev and wk.dtype is f32 and wk.shape == (hd,) and wk.is_contiguous()
+        wk_ptr = wk.data_ptr()
+    if fits and inv_freq is not None:
+        fits = inv_freq.get_device() == dev and inv_freq.dtype is f32 and inv_freq.shape == (hd // 2,) and inv_freq.is_contiguous()
+        freq_ptr = inv_freq.data_ptr()
+    if not fits:
+        _misfit("kv4_prepare", (("qkv", qkv, f32, (N, (nh + 2 * nkv) * hd)), ("q norm weight", wq, f32, (hd,)), ("k norm weight", wk, f32, (hd,)),
+                                ("inv_freq", inv_freq, f32, (hd // 2,)), ("positions", positions, i32, (N,)), ("seq_of", seq_of, i32, (N,)),
+                                ("page table", page_table, i32, table_shape), ("cache pool", pool, torch.uint8, pool.shape),
+                                ("q out", q_out, q_out.dtype, (N, nh * hd))))
     ptr, out = qkv.data_ptr(), q_out.data_ptr()
-    wq_ptr, wk_ptr = None if wq is None else wq.data_ptr(), None if wk is None else wk.data_ptr()
-    for name, p in (("qkv", ptr), ("q out", out), ("q norm weight", wq_ptr or 0), ("k norm weight", wk_ptr or 0)):
-        if p % 16:
-            raise KernelError(f"kv4_prepare: {name} must start on 16 bytes")
+    if (ptr | out | (wq_ptr or 0) | (wk_ptr or 0)) % 16:
+        raise KernelError("kv4_prepare: qkv, q out and the norm weights must start on 16 bytes")
     _guard("core", "kv4_cache", qkv.device, n_pages=pool.shape[0])
     _check(_fn("core", "mv_kv4_prepare")(
-        ptr, wq_ptr, wk_ptr, eps, None if inv_freq is None else inv_freq.data_ptr(), bool(half_split), positions.data_ptr(), seq_of.data_ptr(),
+        ptr, wq_ptr, wk_ptr, eps, freq_ptr, bool(half_split), positions.data_ptr(), seq_of.data_ptr(),
         page_table.data_ptr(), table_shape[1], page_size, pool.data_ptr(), out, dt, N, nh, nkv, hd, _stream()), "mv_kv4_prepare")
     if _profile is not None:
         account(_nbytes(qkv, q_out) + N * nkv * (hd + 8))
@@ -2715,9 +2725,16 @@ def kv4_read(pool: torch.Tensor, page_table, positions, seq_of, k_out: torch.Ten
     if k_out.dtype != v_out.dtype:
         raise KernelError(f"kv4_read: k out is {k_out.dtype} but v out is {v_out.dtype}")
     table_shape = _table_shape(page_table, "kv4_read")
-    dt, i32 = _dt(k_out), torch.int32
-    _need_all("kv4_read", (("cache pool", pool, torch.uint8, pool.shape), ("page table", page_table, i32, table_shape), ("positions", positions, i32, (N,)),
-                           ("seq_of", seq_of, i32, (N,)), ("k out", k_out, k_out.dtype, (N, nkv, hd)), ("v out", v_out, v_out.dtype, (N, nkv, hd))))
+    dt, dev, i32, shape = _dt(k_out), pool.get_device(), torch.int32, (N, nkv, hd)
+    if not (pool.is_contiguous() and _is_current(dev)
+            and page_table.get_device() == dev and page_table.dtype is i32 and page_table.is_contiguous()
+            and positions.get_device() == dev and positions.dtype is i32 and positions.shape == (N,) and positions.is_contiguous()
+            and seq_of.get_device() == dev and seq_of.dtype is i32 and seq_of.shape == (N,) and seq_of.is_contiguous()
+            and k_out.get_device() == dev and k_out.shape == shape and k_out.is_contiguous()
+            and v_out.get_device() == dev and v_out.shape == shape and v_out.is_contiguous()):
+        _misfit("kv4_read", (("cache pool", pool, torch.uint8, pool.shape), ("page table", page_table, i32, table_shape),
+                             ("positions", positions, i32, (N,)), ("seq_of", seq_of, i32, (N,)), ("k out", k_out, k_out.dtype, shape),
+                             ("v out", v_out, v_out.dtype, shape)))
     k_ptr, v_ptr = k_out.data_ptr(), v_out.data_ptr()
     if k_ptr % 16 or v_ptr % 16:
         raise KernelError("kv4_read: k out and v out must start on 16 bytes")
@@ -2770,29 +2787,40 @@ def attention_kv4(q: torch.Tensor, pool: torch.Tensor, page_table, positions, se
         raise KernelError(f"attention_kv4: scale {scale}, expected a positive number")
     if splits is not None and not 1 <= int(splits) <= 1024:
         raise KernelError(f"attention_kv4: {splits} key splits, expected 1..1024")
-    dt, i32 = _dt(q), torch.int32
     rows, W = table_shape = _table_shape(page_table, "attention_kv4")
-    dev = _need_all("attention_kv4", (("q", q, q.dtype, (N, nh * hd)), ("cache pool", pool, torch.uint8, pool.shape),
-                                      ("page table", page_table, i32, table_shape), ("positions", positions, i32, (N,)), ("seq_of", seq_of, i32, (N,)),
-                                      ("cu", cu, i32, (B + 1,)), ("starts", starts, i32, (B,)), ("attention out", out, q.dtype, (N, nh * hd))))
-    if q.data_ptr() % 16 or out.data_ptr() % 16:
+    dt, dev, i32, dtype, shape = _dt(q), q.get_device(), torch.int32, q.dtype, (N, nh * hd)
+    if not (q.shape == shape and q.is_contiguous() and _is_current(dev)
+            and out.get_device() == dev and out.shape == shape and out.is_contiguous()
+            and pool.get_device() == dev and pool.is_contiguous()
+            and page_table.get_device() == dev and page_table.dtype is i32 and page_table.is_contiguous()
+            and positions.get_device() == dev and positions.dtype is i32 and positions.shape == (N,) and positions.is_contiguous()
+            and seq_of.get_device() == dev and seq_of.dtype is i32 and seq_of.shape == (N,) and seq_of.is_contiguous()
+            and cu.get_device() == dev and cu.dtype is i32 and cu.shape == (B + 1,) and cu.is_contiguous()
+            and starts.get_device() == dev and starts.dtype is i32 and starts.shape == (B,) and starts.is_contiguous()):
+        _misfit("attention_kv4", (("q", q, dtype, shape), ("cache pool", pool, torch.uint8, pool.shape), ("page table", page_table, i32, table_shape),
+                                  ("positions", positions, i32, (N,)), ("seq_of", seq_of, i32, (N,)), ("cu", cu, i32, (B + 1,)),
+                                  ("starts", starts, i32, (B,)), ("attention out", out, dtype, shape)))
+    if (q.data_ptr() | out.data_ptr()) % 16:
         raise KernelError("attention_kv4: q and out must start on 16 bytes")
     if B == 0:
         return out
     if rows < B:
         raise KernelError(f"attention_kv4: a page table of {rows} sequences for a step of {B}")
-    max_len = max(host_lens)
-    if max(host_starts) + max_len > W * page_size and max(map(int.__add__, host_starts, host_lens)) > W * page_size:
-        raise KernelError(f"attention_kv4: {max(map(int.__add__, host_starts, host_lens))} tokens in a sequence, the page table reaches {W * page_size}")
-    args = (pool, page_table, page_size, positions, seq_of, starts, out, nh, nkv, hd, float(scale), int(window), ws)
+    max_len, reach = max(host_lens), max(host_starts)
+    reach += max_len
+    if reach > W * page_size:
+        reach = max(map(int.__add__, host_starts, host_lens))
+        if reach > W * page_size:
+            raise KernelError(f"attention_kv4: {reach} tokens in a sequence, the page table reaches {W * page_size}")
+    args = (pool, page_table, W, page_size, positions, seq_of, starts, out, nh, nkv, hd, scale, window, ws)
     if max_len <= KV4_DIRECT_TOKENS:
-        _attention_kv4_direct(q, *args, 0, N, max_len, max(host_starts) + max_len, splits, dt, dev)
+        _attention_kv4_direct(q, *args, 0, N, max_len, reach, splits, dt, dev)
         return out
     n0 = 0
     for b0, b1, pages in kv4_runs(host_starts, host_lens, window, page_size, 2 * nkv * page_size * hd * q.element_size()):
         n1 = n0 + sum(host_lens[b0:b1])
         if pages == 0:
-            _attention_kv4_direct(q, *args, n0, n1, max(host_lens[b0:b1]), max(host_starts) + max_len, splits, dt, dev)
+            _attention_kv4_direct(q, *args, n0, n1, max(host_lens[b0:b1]), reach, splits, dt, dev)
         else:
             _attention_kv4_pages(q, *args, cu, b0, b1, n0, n1, pages, host_lens)
         n0 = n1
@@ -2835,13 +2863,12 @@ def attention_kv4_decode_plan(N: int, nh: int, nkv: int, hd: int, max_len: int):
     return nt, head_tiles, heads, tokens, KV4_DECODE_WAVES * resident * n_sms()
 
 
-def _attention_kv4_direct(q, pool, page_table, page_size, positions, seq_of, starts, out, nh, nkv, hd, scale, window, ws, n0, n1, max_len, reach,
-                          splits, dt, dev):
+def _attention_kv4_direct(q, pool, page_table, W, page_size, positions, seq_of, starts, out, nh, nkv, hd, scale, window, ws, n0, n1, max_len,
+                          reach, splits, dt, dev):
     """The query rows n0 .. n1 - 1, in runs of at most ``max_len`` of a sequence, over the codes themselves.  ``reach``: rows of the
     longest sequence."""
-    N, W = n1 - n0, page_table.shape[1]
+    N = n1 - n0
     row = nh * hd * (2 if dt == BF16 else 4) * n0
-    where = (q.data_ptr() + row, pool.data_ptr(), page_table.data_ptr(), W, page_size, positions.data_ptr() + 4 * n0, seq_of.data_ptr() + 4 * n0)
     if dt == BF16 and page_size >= 16:                           # attention_kv4_decode_supported
         nt, head_tiles, heads, tokens, blocks = attention_kv4_decode_plan(N, nh, nkv, hd, max_len)
         pairs, piece = nkv * head_tiles, 0
@@ -2849,19 +2876,18 @@ def _attention_kv4_direct(q, pool, page_table, page_size, positions, seq_of, sta
         if splits is not None:
             piece = -(-(-(-reach // 64)) // int(splits))
             grid = N * pairs * (-(-(reach // 64 + 2) // piece))
-        elif W * page_size <= 256:                               # one piece is all there can be
-            grid = N * pairs
         if grid > 0x7fffffff:
             raise KernelError(f"attention_kv4: {N} tokens and {nkv} kv heads make {grid} blocks")
-        part_o = ws.get("attn_part_o", (grid * 4 * nt * hd,), torch.float32)
-        part_ml = ws.get("attn_part_ml", (grid * 4 * nt * 2,), torch.float32)
-        tickets = ws.get_zeroed("attn_tickets", (N * pairs,), torch.int32)
+        parts = grid * 4 * nt
+        part_ml = ws.get("kv4_parts", (parts * (hd + 2),), torch.float32).data_ptr()
+        tickets = ws.get_zeroed("attn_tickets", (N * pairs,), torch.int32).data_ptr()
         flag = _error_flags.get(dev)
-        _guard("bf16", "attention_kv4_decode", q.device, n_pages=pool.shape[0])
+        if DEBUG_CHECKS:
+            _guard("bf16", "attention_kv4_decode", q.device, n_pages=pool.shape[0])
         _check(_fn("bf16", "mv_attention_kv4_decode")(
-            *where, starts.data_ptr(), out.data_ptr() + row, part_o.data_ptr(), part_ml.data_ptr(), tickets.data_ptr(), N, nh, nkv, hd, scale,
-            window, nt, head_tiles, heads, tokens, piece, blocks, grid, (_error_flag(q.device) if flag is None else flag).data_ptr(), _stream()),
-            "mv_attention_kv4_decode")
+            q.data_ptr() + row, pool.data_ptr(), page_table.data_ptr(), W, page_size, positions.data_ptr() + 4 * n0, seq_of.data_ptr() + 4 * n0,
+            starts.data_ptr(), out.data_ptr() + row, part_ml + 8 * parts, part_ml, tickets, N, nh, nkv, hd, scale, window, nt, head_tiles, heads,
+            tokens, piece, blocks, grid, (_error_flag(q.device) if flag is None else flag).data_ptr(), _stream()), "mv_attention_kv4_decode")
         return
     gt, head_tiles, auto = attention_kv4_plan(N, nh, nkv, W * page_size)
     splits = auto if splits is None else int(splits)
@@ -2873,19 +2899,20 @@ def _attention_kv4_direct(q, pool, page_table, page_size, positions, seq_of, sta
         part_ml = ws.get("attn_part_ml", (N * nh * splits * 2,), torch.float32).data_ptr()
         tickets = ws.get_zeroed("attn_tickets", (N * nkv * head_tiles,), torch.int32).data_ptr()
     _guard("core", "kv4_cache", q.device, n_pages=pool.shape[0])
-    _check(_fn("core", "mv_attention_kv4")(*where, out.data_ptr() + row, dt, part_o, part_ml, tickets, N, nh, nkv, hd, scale, window, splits, gt,
-                                           head_tiles, _stream()), "mv_attention_kv4")
+    _check(_fn("core", "mv_attention_kv4")(
+        q.data_ptr() + row, pool.data_ptr(), page_table.data_ptr(), W, page_size, positions.data_ptr() + 4 * n0, seq_of.data_ptr() + 4 * n0,
+        out.data_ptr() + row, dt, part_o, part_ml, tickets, N, nh, nkv, hd, scale, window, splits, gt, head_tiles, _stream()), "mv_attention_kv4")
 
 
-def _attention_kv4_pages(q, pool, page_table, page_size, positions, seq_of, starts, out, nh, nkv, hd, scale, window, ws, cu, b0, b1, n0, n1, pages,
+def _attention_kv4_pages(q, pool, page_table, W, page_size, positions, seq_of, starts, out, nh, nkv, hd, scale, window, ws, cu, b0, b1, n0, n1, pages,
                          host_lens):
     """Sequences b0 .. b1 - 1: their pages are read back into a pool of their own, which the attention kernels of many tokens read."""
-    W, n_seqs = page_table.shape[1], b1 - b0
+    n_seqs = b1 - b0
     if n_seqs > 65535 or nkv > 65535:
         raise KernelError(f"attention_kv4: {n_seqs} sequences and {nkv} kv heads in one launch; each may be 65535 at most")
     # (a power of two pages: the pool keeps its shape, and with it its tensor map, as sequences grow)
     read = ws.get("kv4_pages", (1 << (pages - 1).bit_length(), 2, nkv, page_size, hd), q.dtype)
-    table = ws.get("kv4_table", tuple(page_table.shape), torch.int32)
+    table = ws.get("kv4_table", (page_table.shape[0], W), torch.int32)
     cu_run, starts_run, table_run = cu[b0:b1 + 1], starts[b0:b1], table[b0:b1]
     _guard("core", "kv4_cache", q.device, n_pages=pool.shape[0])
     _check(_fn("core", "mv_kv4_read_pages")(
