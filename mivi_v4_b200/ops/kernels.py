@@ -137,6 +137,7 @@ _SIGNATURES = {
         "mv_attention_decode_tc": [_P, _P, _Q, _P, _I, _P, _P, _P, _P, _P, _I, _I, _I, _F, _I, _P, _P],
         "mv_attention_prefill_tc": [_P, _P, _Q, _P, _I, _P, _P, _P, _I, _I, _I, _I, _F, _P, _P],
         "mv_attention_kv4_decode": [_P, _P, _P, _I, _I, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _F, _I, _I, _I, _I, _I, _I, _I, _I, _P, _P],
+        "mv_attention_kv4_prefill": [_P, _P, _P, _I, _I, _P, _P, _P, _P, _P, _P, _I, _I, _I, _F, _I, _I, _I, _P, _P],
         "mv_latent_attention_decode": [_P, _P, _Q, _P, _I, _I, _P, _P, _P, _P, _I, _I, _I, _I, _F, _I, _I, _P, _P, _P, _P],
         "mv_latent_query": [_P, _I, _I, _P, _P, _P, _I, _I, _I, _I, _I, _F, _P],
         "mv_latent_gather": [_P, _Q, _P, _I, _I, _P, _P, _I, _I, _I, _I, _P, _P, _I, _P],
@@ -2048,7 +2049,7 @@ _error_mirrors = {}
 _ERROR_CODES = (((1, 3), "gemm_tc.cu"), ((5, 5), "gemm_tc.cu"), ((11, 21), "attention_prefill_tc.cu"), ((30, 40), "attention_decode_tc.cu"),
                 ((45, 45), "latent_attention_decode.cu"), ((51, 63), "latent_attention_tc.cu"), ((71, 76), "gemm_f32_tc.cu"),
                 ((81, 93), "attention_sink_tc.cu"), ((101, 103), "gemm_tc_swap.cu"), ((111, 115), "gemm_tc_pair.cu"),
-                ((150, 151), "attention_kv4_decode.cu"))
+                ((150, 151), "attention_kv4_decode.cu"), ((160, 171), "attention_kv4_prefill.cu"))
 # the products' roles, by the last digit
 _ERROR_ROLES = {1: "the TMA producer", 2: "the MMA issuer", 3: "the epilogue", 5: "the MMA issuer (for the epilogue)"}
 
@@ -2817,9 +2818,12 @@ def attention_kv4(q: torch.Tensor, pool: torch.Tensor, page_table, positions, se
         _attention_kv4_direct(q, *args, 0, N, max_len, reach, splits, dt, dev)
         return out
     n0 = 0
-    for b0, b1, pages in kv4_runs(host_starts, host_lens, window, page_size, 2 * nkv * page_size * hd * q.element_size()):
+    fused = dt == BF16 and hd == 64                              # attention_kv4_prefill_supported
+    for b0, b1, pages in kv4_runs(host_starts, host_lens, window, page_size, 0 if fused else 2 * nkv * page_size * hd * q.element_size()):
         n1 = n0 + sum(host_lens[b0:b1])
-        if pages == 0:
+        if pages and fused:
+            _attention_kv4_prefill(q, pool, page_table, W, page_size, cu, starts, out, nh, nkv, scale, window, ws, b0, b1, host_starts, host_lens, dev)
+        elif pages == 0:
             _attention_kv4_direct(q, *args, n0, n1, max(host_lens[b0:b1]), reach, splits, dt, dev)
         else:
             _attention_kv4_pages(q, *args, cu, b0, b1, n0, n1, pages, host_lens)
@@ -2902,6 +2906,65 @@ def _attention_kv4_direct(q, pool, page_table, W, page_size, positions, seq_of, 
     _check(_fn("core", "mv_attention_kv4")(
         q.data_ptr() + row, pool.data_ptr(), page_table.data_ptr(), W, page_size, positions.data_ptr() + 4 * n0, seq_of.data_ptr() + 4 * n0,
         out.data_ptr() + row, dt, part_o, part_ml, tickets, N, nh, nkv, hd, scale, window, splits, gt, head_tiles, _stream()), "mv_attention_kv4")
+
+
+def attention_kv4_prefill_supported(dtype: torch.dtype, hd: int) -> bool:
+    """What the tcgen05 kernel over the codes takes: bfloat16 and heads of 64 (pages of any size, windows)."""
+    return dtype == torch.bfloat16 and hd == 64
+
+
+KV4_PREFILL_MOST = 1024             # most sequences, and most tiles of 256 rows, of a launch (attention_kv4_prefill.cu)
+
+
+@functools.lru_cache(maxsize=256)
+def attention_kv4_prefill_plan(starts: tuple, lens: tuple, group: int, nkv: int, window: int):
+    """[(sequences, tiles, whether a block takes whole tiles and kv heads, blocks)] for the launches over neighbouring sequences that bring
+    ``lens`` tokens from ``starts`` on.  A tile is 256 rows, tokens by the heads of a kv head.  Costs are counted in key blocks of 128, 2 us
+    each: a whole tile's beginning and end take about one and a half more, a tile that is shared among blocks about five for each of them
+    (its parts are written, fetched and put together).  The way that ends earlier is taken."""
+    plan, b, sms = [], 0, n_sms()
+    while b < len(lens):
+        sizes, end = [], b
+        while end < len(lens) and end - b < KV4_PREFILL_MOST:
+            rows = lens[end] * group
+            if len(sizes) - (-rows // 256) > KV4_PREFILL_MOST:
+                break
+            for r in range(0, rows, 256):
+                last, first = starts[end] + (min(rows, r + 256) - 1) // group, starts[end] + r // group
+                sizes.append(last // 128 + 1 - (max(0, first - window + 1) // 128 if window > 0 else 0))
+            end += 1
+        if end == b:
+            raise KernelError(f"attention_kv4: {lens[b]} tokens of one sequence by {group} heads a kv head in one step; at most "
+                              f"{KV4_PREFILL_MOST * 256} rows")
+        units, total = len(sizes) * nkv, sum(sizes) * nkv
+        blocks = min(sms, units)
+        busy = [0.0] * blocks
+        for i in range(units if units <= 8 * sms else 0):        # as the kernel hands them out: the last first, back and forth
+            lap, at = divmod(i, blocks)
+            busy[blocks - 1 - at if lap & 1 else at] += sizes[(units - 1 - i) // nkv] + 1.5
+        whole = max(busy) if units <= 8 * sms else (total + 1.5 * units) / sms
+        shares = max(1, min(sms, total // 4))
+        shared = total / shares + 5.0 * (units / shares + 1.0)
+        plan.append((end - b, len(sizes), whole <= shared, blocks if whole <= shared else shares))
+        b = end
+    return plan
+
+
+def _attention_kv4_prefill(q, pool, page_table, W, page_size, cu, starts, out, nh, nkv, scale, window, ws, b0, b1, host_starts, host_lens, dev):
+    """Sequences b0 .. b1 - 1, many tokens each, over the codes on tcgen05."""
+    flag = _error_flags.get(dev)
+    for n_seqs, tiles, whole, grid in attention_kv4_prefill_plan(tuple(host_starts[b0:b1]), tuple(host_lens[b0:b1]), nh // nkv, nkv, window):
+        parts = tickets = None
+        if not whole:
+            parts = ws.get("kv4_tile_parts", (2 * grid * 256 * 66,), torch.float32).data_ptr()
+            tickets = ws.get_zeroed("kv4_tile_tickets", (tiles * nkv,), torch.int32).data_ptr()
+        if DEBUG_CHECKS:
+            _guard("bf16", "attention_kv4_prefill", q.device, n_pages=pool.shape[0])
+        _check(_fn("bf16", "mv_attention_kv4_prefill")(
+            q.data_ptr(), pool.data_ptr(), page_table.data_ptr() + 4 * W * b0, W, page_size, cu.data_ptr() + 4 * b0, starts.data_ptr() + 4 * b0,
+            out.data_ptr(), parts, None if whole else parts + 2 * grid * 256 * 64 * 4, tickets, n_seqs, nh, nkv, scale, window, whole, grid,
+            (_error_flag(q.device) if flag is None else flag).data_ptr(), _stream()), "mv_attention_kv4_prefill")
+        b0 += n_seqs
 
 
 def _attention_kv4_pages(q, pool, page_table, W, page_size, positions, seq_of, starts, out, nh, nkv, hd, scale, window, ws, cu, b0, b1, n0, n1, pages,
