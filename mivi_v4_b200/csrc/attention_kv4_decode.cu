@@ -87,15 +87,15 @@ struct KdShape {
     static constexpr int BARS = RING > MERGE ? RING : MERGE, SMEM = BARS + KD_WARPS * STAGES * 8;
 };
 
-// EXACT: HDP is the head size.  A column is token c / heads and head h0 + c % heads of the kv head's group, heads = min(group, 4 NT).  Only a token
+// EXACT: HDP is the head size.  The N rows are those from n0 of the step on (cu counts from its first).  A column is token c / heads and head h0 + c % heads of the kv head's group, heads = min(group, 4 NT).  Only a token
 // whose place in its sequence's run is a multiple of tokens_per_tile begins a tile.  Block b works on kv head and head tile b % pairs of
 // piece b / pairs, counted over the tiles of columns.  piece: tiles of 64 keys in one; 0: such that there are ``blocks`` of them.
 template <int HDP, bool EXACT, int NT>
 __global__ void __launch_bounds__(KD_WARPS * 32, KdShape<HDP, NT>::RESIDENT)
 attention_kv4_decode_kernel(const __nv_bfloat16* __restrict__ q, const unsigned char* __restrict__ pool, const int* __restrict__ page_table,
                             int table_stride, int page_shift, const int* __restrict__ positions, const int* __restrict__ seq_of,
-                            const int* __restrict__ starts, __nv_bfloat16* __restrict__ o, float* __restrict__ part_o,
-                            float* __restrict__ part_ml, int* __restrict__ tickets, int N, int nh, int nkv, int hd_, float scale_log2, int window,
+                            const int* __restrict__ cu, int n0, const int* __restrict__ starts, __nv_bfloat16* __restrict__ o,
+                            float* __restrict__ part_o, float* __restrict__ part_ml, int* __restrict__ tickets, int N, int tiles, int nh, int nkv, int hd_, float scale_log2, int window,
                             int head_tiles, int heads, int tokens_per_tile, int piece, int blocks, int* __restrict__ err) {
     mv_pdl_begin();
     using Shape = KdShape<HDP, NT>;
@@ -115,8 +115,9 @@ attention_kv4_decode_kernel(const __nv_bfloat16* __restrict__ q, const unsigned 
         row_pos = positions[r];
         row_tokens = 1;
         if (tokens_per_tile > 1) {
-            if ((row_pos - starts[row_seq]) % tokens_per_tile) return 0;
-            while (row_tokens < tokens_per_tile && r + row_tokens < N && seq_of[r + row_tokens] == row_seq) ++row_tokens;
+            const int in_tile = (row_pos - starts[row_seq]) % tokens_per_tile;
+            if (in_tile && r) return 0;                          // (the launch's first row begins one wherever it stands)
+            row_tokens = min(tokens_per_tile - in_tile, min(N, cu[row_seq + 1] - n0) - r);
         }
         return (row_pos + row_tokens - 1) / KD_KEYS + 1 - (window > 0 ? max(0, row_pos - window + 1) / KD_KEYS : 0);
     };
@@ -150,7 +151,7 @@ attention_kv4_decode_kernel(const __nv_bfloat16* __restrict__ q, const unsigned 
                 mine = tiles_at(threadIdx.x);
             }
             // (half a piece a tile of columns is lost where its keys end: as many blocks are left to it)
-            const int aim = max(blocks / 2, blocks - (N * pairs + 1) / 2);
+            const int aim = max(blocks / 2, blocks - (tiles * pairs + 1) / 2);
             piece = max(KD_WARPS, (int)((all * pairs + aim - 1) / aim));
         }
         if (threadIdx.x == 0) found[0] = -1;
@@ -606,8 +607,8 @@ int kd_launch(dim3 grid, cudaStream_t stream, A... args) {
 // pieces in all); ``grid`` bounds the pieces times kv heads and head tiles: blocks + N * nkv * head_tiles where piece is 0.
 // part_o [grid, 4 nt, hd] and part_ml [grid, 4 nt, 2] float32, tickets [N, nkv * head_tiles] (zero).
 MV_API int mv_attention_kv4_decode(const void* q, const void* pool, const int* page_table, int table_stride, int page_size,
-                                   const int* positions, const int* seq_of, const int* starts, void* o, float* part_o, float* part_ml,
-                                   int* tickets, int N, int nh, int nkv, int hd, float scale, int window, int nt, int head_tiles, int heads,
+                                   const int* positions, const int* seq_of, const int* cu, int n0, const int* starts, void* o,
+                                   float* part_o, float* part_ml, int* tickets, int N, int tiles, int nh, int nkv, int hd, float scale, int window, int nt, int head_tiles, int heads,
                                    int tokens_per_tile, int piece, int blocks, int grid, int* err, cudaStream_t stream) {
     if (N <= 0) return 0;
     if (hd % 8 || hd < 8 || hd > KV4_MAX_HEAD_DIM || nkv < 1 || nh % nkv || page_size < 16 || (page_size & (page_size - 1)) || blocks < 1 ||
@@ -618,7 +619,7 @@ MV_API int mv_attention_kv4_decode(const void* q, const void* pool, const int* p
     while ((1 << page_shift) < page_size) ++page_shift;
 #define MV_GO(HDP, EXACT, NT)                                                                                                            \
     return kd_launch<HDP, EXACT, NT>(dim3(grid), stream, (const __nv_bfloat16*)q, (const unsigned char*)pool, page_table, table_stride,   \
-                                     page_shift, positions, seq_of, starts, (__nv_bfloat16*)o, part_o, part_ml, tickets, N, nh, nkv, hd,  \
+                                     page_shift, positions, seq_of, cu, n0, starts, (__nv_bfloat16*)o, part_o, part_ml, tickets, N, tiles, nh, nkv, hd, \
                                      scale * 1.4426950408889634f, window, head_tiles, heads, tokens_per_tile, piece, blocks, err)
     if (hd <= 64) {
         if (hd == 64) {

@@ -237,7 +237,8 @@ attention_kv4_prefill_kernel(const __nv_bfloat16* __restrict__ q, const unsigned
     if (tid == 0) before[n_tiles] = n_blocks;
     __syncthreads();
     // shares: block c works on what lies from begin_of(c) to begin_of(c + 1); a tile's kv head takes KQ_EXTRA and its key blocks
-    const int total = (n_blocks + KQ_EXTRA * n_tiles) * nkv, C = gridDim.x;
+    // (a share is one at least: the blocks of a tile are counted, and each of them has a part)
+    const int total = (n_blocks + KQ_EXTRA * n_tiles) * nkv, C = whole ? (int)gridDim.x : max(1, min((int)gridDim.x, total));
     const double share_of = (double)total / (double)C, per_share = (double)C / (double)total;
     auto begin_of = [&](int c) { return c >= C ? total : (int)((double)c * share_of); };
     auto block_of = [&](int x) {
@@ -320,9 +321,15 @@ attention_kv4_prefill_kernel(const __nv_bfloat16* __restrict__ q, const unsigned
             auto fetch = [&](uint4 (&w)[2], int at) {
                 w[0] = w[1] = make_uint4(0u, 0u, 0u, 0u);
                 if (from != nullptr) {
-                    const uint4* x = reinterpret_cast<const uint4*>(from + at + row * (HD / 2));
-                    w[0] = x[0];
-                    w[1] = x[1];
+                    if (page_shift) {
+                        const uint4* x = reinterpret_cast<const uint4*>(from + at + row * (HD / 2));
+                        w[0] = x[0];
+                        w[1] = x[1];
+                    } else {                                     // (pages of one token are 72 bytes a kv head: 8 is all they are aligned to)
+                        const uint2* x = reinterpret_cast<const uint2*>(from + at);
+                        w[0] = make_uint4(x[0].x, x[0].y, x[1].x, x[1].y);
+                        w[1] = make_uint4(x[2].x, x[2].y, x[3].x, x[3].y);
+                    }
                 }
             };
             auto fetch_numbers = [&]() { np = from != nullptr ? *reinterpret_cast<const uint2*>(from + page_size * HD + row * 8) : make_uint2(0u, 0u); };

@@ -136,7 +136,7 @@ _SIGNATURES = {
                                      _P, _P],
         "mv_attention_decode_tc": [_P, _P, _Q, _P, _I, _P, _P, _P, _P, _P, _I, _I, _I, _F, _I, _P, _P],
         "mv_attention_prefill_tc": [_P, _P, _Q, _P, _I, _P, _P, _P, _I, _I, _I, _I, _F, _P, _P],
-        "mv_attention_kv4_decode": [_P, _P, _P, _I, _I, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _F, _I, _I, _I, _I, _I, _I, _I, _I, _P, _P],
+        "mv_attention_kv4_decode": [_P, _P, _P, _I, _I, _P, _P, _P, _I, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _F, _I, _I, _I, _I, _I, _I, _I, _I, _P, _P],
         "mv_attention_kv4_prefill": [_P, _P, _P, _I, _I, _P, _P, _P, _P, _P, _P, _I, _I, _I, _F, _I, _I, _I, _P, _P],
         "mv_latent_attention_decode": [_P, _P, _Q, _P, _I, _I, _P, _P, _P, _P, _I, _I, _I, _I, _F, _I, _I, _P, _P, _P, _P],
         "mv_latent_query": [_P, _I, _I, _P, _P, _P, _I, _I, _I, _I, _I, _F, _P],
@@ -2747,18 +2747,25 @@ def kv4_read(pool: torch.Tensor, page_table, positions, seq_of, k_out: torch.Ten
     return k_out, v_out
 
 
-KV4_DIRECT_TOKENS = 16              # tokens a sequence up to which a step's queries read the codes themselves
+# Tokens a sequence up to which a step's queries read the codes themselves, in a kernel made for few.  Heads of 64, 32 / 8 of them: 16 sequences
+# of 6 tokens behind 3,000 take 29 us there and 51 us in the tcgen05 kernel, 8 of 9 behind 2,000 22 and 31, 8 of 20 39 and 31.
+KV4_DIRECT_TOKENS = 16
+# Where many tokens have their cache read back first, these few do better without it behind a long context: at most so many in the step,
+# each behind at least so many keys (``attention_kv4``).
+KV4_FAR_TOKENS, KV4_FAR_KEYS = 256, 32
 KV4_READ_BYTES = 1 << 30            # most of the cache that is read back at a time, unless one sequence alone is more
 
 
-def kv4_runs(starts, lens, window: int, page_size: int, page_bytes: int):
+def kv4_runs(starts, lens, window: int, page_size: int, page_bytes: int, far: bool = False):
     """How a step's sequences are attended to: [(first sequence, one past the last, pages to read back, 0 for none)].  Neighbours
     that bring at most ``KV4_DIRECT_TOKENS`` tokens each read the codes themselves, together; the others' pages (``page_bytes``
-    each once they are read back) are read back first, for as many neighbours together as ``KV4_READ_BYTES`` holds."""
+    each once they are read back) are read back first, for as many neighbours together as ``KV4_READ_BYTES`` holds.  ``far``: so do the
+    sequences of a step of at most ``KV4_FAR_TOKENS`` tokens that see ``KV4_FAR_KEYS`` cached keys for each that they bring."""
+    far = far and sum(lens) <= KV4_FAR_TOKENS
     runs = []
     for b, (s, n) in enumerate(zip(starts, lens)):
         pages = 0
-        if n > KV4_DIRECT_TOKENS:
+        if n > KV4_DIRECT_TOKENS and not (far and (min(s, window) if window > 0 else s) >= KV4_FAR_KEYS * n):
             first = max(0, s - window + 1) // page_size if window > 0 else 0
             pages = -(-(s + n) // page_size) - first
         if runs and (runs[-1][2] > 0) == (pages > 0) and (runs[-1][2] + pages) * page_bytes <= KV4_READ_BYTES:
@@ -2814,17 +2821,22 @@ def attention_kv4(q: torch.Tensor, pool: torch.Tensor, page_table, positions, se
         if reach > W * page_size:
             raise KernelError(f"attention_kv4: {reach} tokens in a sequence, the page table reaches {W * page_size}")
     args = (pool, page_table, W, page_size, positions, seq_of, starts, out, nh, nkv, hd, scale, window, ws)
-    if max_len <= KV4_DIRECT_TOKENS:
-        _attention_kv4_direct(q, *args, 0, N, max_len, reach, splits, dt, dev)
+    fused = attention_kv4_prefill_supported(dtype, hd)
+    codes = not fused and attention_kv4_decode_supported(dtype, page_size)
+    # (head sizes that no tensor-core kernel of many tokens takes, 8 / 2 heads of 256: 2,048 tokens of a prompt take 296 us over the codes in
+    # launches of 256 rows, 3,840 us read back)
+    if max_len <= KV4_DIRECT_TOKENS or (codes and not attention_prefill_supported(dtype, hd)):
+        _attention_kv4_direct(q, *args, cu, 0, N, B, max_len, reach, splits, dt, dev)
         return out
     n0 = 0
-    fused = dt == BF16 and hd == 64                              # attention_kv4_prefill_supported
-    for b0, b1, pages in kv4_runs(host_starts, host_lens, window, page_size, 0 if fused else 2 * nkv * page_size * hd * q.element_size()):
+    # (far: heads of 128, 16 / 4 of them, 20 tokens behind 8,000: 30 us over the codes, 240 us read back; 64: 51 and 240)
+    for b0, b1, pages in kv4_runs(host_starts, host_lens, window, page_size, 0 if fused else 2 * nkv * page_size * hd * q.element_size(),
+                                  codes):
         n1 = n0 + sum(host_lens[b0:b1])
         if pages and fused:
             _attention_kv4_prefill(q, pool, page_table, W, page_size, cu, starts, out, nh, nkv, scale, window, ws, b0, b1, host_starts, host_lens, dev)
         elif pages == 0:
-            _attention_kv4_direct(q, *args, n0, n1, max(host_lens[b0:b1]), reach, splits, dt, dev)
+            _attention_kv4_direct(q, *args, cu, n0, n1, b1 - b0, max(host_lens[b0:b1]), reach, splits, dt, dev)
         else:
             _attention_kv4_pages(q, *args, cu, b0, b1, n0, n1, pages, host_lens)
         n0 = n1
@@ -2847,6 +2859,7 @@ def attention_kv4_decode_supported(dtype: torch.dtype, page_size: int) -> bool:
     return dtype == torch.bfloat16 and page_size >= 16
 
 
+KV4_DIRECT_ROWS = 256               # most rows of a launch: each of its blocks looks through them for its own work
 KV4_DECODE_WAVES = 1                # how many times over the pieces of a step fill the device
 
 
@@ -2867,19 +2880,26 @@ def attention_kv4_decode_plan(N: int, nh: int, nkv: int, hd: int, max_len: int):
     return nt, head_tiles, heads, tokens, KV4_DECODE_WAVES * resident * n_sms()
 
 
-def _attention_kv4_direct(q, pool, page_table, W, page_size, positions, seq_of, starts, out, nh, nkv, hd, scale, window, ws, n0, n1, max_len,
-                          reach, splits, dt, dev):
-    """The query rows n0 .. n1 - 1, in runs of at most ``max_len`` of a sequence, over the codes themselves.  ``reach``: rows of the
-    longest sequence."""
+def _attention_kv4_direct(q, pool, page_table, W, page_size, positions, seq_of, starts, out, nh, nkv, hd, scale, window, ws, cu, n0, n1, n_seqs,
+                          max_len, reach, splits, dt, dev):
+    """The query rows n0 .. n1 - 1, in ``n_seqs`` runs of at most ``max_len`` of a sequence, over the codes themselves.  ``reach``: rows
+    of the longest sequence."""
     N = n1 - n0
     row = nh * hd * (2 if dt == BF16 else 4) * n0
-    if dt == BF16 and page_size >= 16:                           # attention_kv4_decode_supported
+    if N > KV4_DIRECT_ROWS:
+        for a in range(n0, n1, KV4_DIRECT_ROWS):
+            _attention_kv4_direct(q, pool, page_table, W, page_size, positions, seq_of, starts, out, nh, nkv, hd, scale, window, ws, cu, a,
+                                  min(a + KV4_DIRECT_ROWS, n1), n_seqs, max_len, reach, splits, dt, dev)
+        return
+    if attention_kv4_decode_supported(q.dtype, page_size):
         nt, head_tiles, heads, tokens, blocks = attention_kv4_decode_plan(N, nh, nkv, hd, max_len)
         pairs, piece = nkv * head_tiles, 0
-        grid = blocks + N * pairs
+        # tiles of columns, at most: one for so many tokens, and for what is left of each run and of one that the launch begins within
+        tiles = N if tokens == 1 else min(N, N // tokens + n_seqs + 1)
+        grid = blocks + tiles * pairs
         if splits is not None:
             piece = -(-(-(-reach // 64)) // int(splits))
-            grid = N * pairs * (-(-(reach // 64 + 2) // piece))
+            grid = tiles * pairs * (-(-(reach // 64 + 2) // piece))
         if grid > 0x7fffffff:
             raise KernelError(f"attention_kv4: {N} tokens and {nkv} kv heads make {grid} blocks")
         parts = grid * 4 * nt
@@ -2890,8 +2910,8 @@ def _attention_kv4_direct(q, pool, page_table, W, page_size, positions, seq_of, 
             _guard("bf16", "attention_kv4_decode", q.device, n_pages=pool.shape[0])
         _check(_fn("bf16", "mv_attention_kv4_decode")(
             q.data_ptr() + row, pool.data_ptr(), page_table.data_ptr(), W, page_size, positions.data_ptr() + 4 * n0, seq_of.data_ptr() + 4 * n0,
-            starts.data_ptr(), out.data_ptr() + row, part_ml + 8 * parts, part_ml, tickets, N, nh, nkv, hd, scale, window, nt, head_tiles, heads,
-            tokens, piece, blocks, grid, (_error_flag(q.device) if flag is None else flag).data_ptr(), _stream()), "mv_attention_kv4_decode")
+            cu.data_ptr(), n0, starts.data_ptr(), out.data_ptr() + row, part_ml + 8 * parts, part_ml, tickets, N, tiles, nh, nkv, hd, scale, window,
+            nt, head_tiles, heads, tokens, piece, blocks, grid, (_error_flag(q.device) if flag is None else flag).data_ptr(), _stream()), "mv_attention_kv4_decode")
         return
     gt, head_tiles, auto = attention_kv4_plan(N, nh, nkv, W * page_size)
     splits = auto if splits is None else int(splits)
