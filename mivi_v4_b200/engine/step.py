@@ -57,6 +57,10 @@ class Workspace:
     def get_zeroed(self, name: str, shape: Sequence[int], dtype: torch.dtype) -> torch.Tensor:
         """Like ``get``, but the buffer is zero when it is first handed out (and
         after it had to grow).  For scratch that its kernels leave zeroed."""
+        vkey = (name, dtype, tuple(shape))
+        view = self._views.get(vkey)
+        if view is not None:
+            return view
         n = 1
         for s in shape:
             n *= int(s)
@@ -68,7 +72,11 @@ class Workspace:
             self.generation += 1
             for k in [k for k in self._views if k[0] == name and k[1] == dtype]:
                 del self._views[k]
-        return buf[:n].view(*shape)
+        if len(self._views) > 4096:
+            self._views.clear()
+        view = buf[:n].view(*shape)
+        self._views[vkey] = view
+        return view
 
     def stage(self, name: str, values) -> torch.Tensor:
         """Copy integers (a list or a numpy array) to the device buffer ``name``

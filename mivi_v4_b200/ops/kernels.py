@@ -2709,7 +2709,8 @@ def kv4_prepare(qkv: torch.Tensor, wq: Optional[torch.Tensor], wk: Optional[torc
     ptr, out = qkv.data_ptr(), q_out.data_ptr()
     if (ptr | out | (wq_ptr or 0) | (wk_ptr or 0)) % 16:
         raise KernelError("kv4_prepare: qkv, q out and the norm weights must start on 16 bytes")
-    _guard("core", "kv4_cache", qkv.device, n_pages=pool.shape[0])
+    if DEBUG_CHECKS:
+        _guard("core", "kv4_cache", qkv.device, n_pages=pool.shape[0])
     _check(_fn("core", "mv_kv4_prepare")(
         ptr, wq_ptr, wk_ptr, eps, freq_ptr, bool(half_split), positions.data_ptr(), seq_of.data_ptr(),
         page_table.data_ptr(), table_shape[1], page_size, pool.data_ptr(), out, dt, N, nh, nkv, hd, _stream()), "mv_kv4_prepare")
@@ -2739,7 +2740,8 @@ def kv4_read(pool: torch.Tensor, page_table, positions, seq_of, k_out: torch.Ten
     k_ptr, v_ptr = k_out.data_ptr(), v_out.data_ptr()
     if k_ptr % 16 or v_ptr % 16:
         raise KernelError("kv4_read: k out and v out must start on 16 bytes")
-    _guard("core", "kv4_cache", pool.device, n_pages=pool.shape[0])
+    if DEBUG_CHECKS:
+        _guard("core", "kv4_cache", pool.device, n_pages=pool.shape[0])
     _check(_fn("core", "mv_kv4_read")(pool.data_ptr(), page_table.data_ptr(), table_shape[1], page_size, positions.data_ptr(), seq_of.data_ptr(),
                                       k_ptr, v_ptr, dt, N, nkv, hd, _stream()), "mv_kv4_read")
     if _profile is not None:
@@ -2820,12 +2822,16 @@ def attention_kv4(q: torch.Tensor, pool: torch.Tensor, page_table, positions, se
         reach = max(map(int.__add__, host_starts, host_lens))
         if reach > W * page_size:
             raise KernelError(f"attention_kv4: {reach} tokens in a sequence, the page table reaches {W * page_size}")
+    if max_len <= KV4_DIRECT_TOKENS:
+        _attention_kv4_direct(q, pool, page_table, W, page_size, positions, seq_of, starts, out, nh, nkv, hd, scale, window, ws, cu, 0, N, B, max_len,
+                              reach, splits, dt, dev)
+        return out
     args = (pool, page_table, W, page_size, positions, seq_of, starts, out, nh, nkv, hd, scale, window, ws)
     fused = attention_kv4_prefill_supported(dtype, hd)
     codes = not fused and attention_kv4_decode_supported(dtype, page_size)
     # (head sizes that no tensor-core kernel of many tokens takes, 8 / 2 heads of 256: 2,048 tokens of a prompt take 296 us over the codes in
     # launches of 256 rows, 3,840 us read back)
-    if max_len <= KV4_DIRECT_TOKENS or (codes and not attention_prefill_supported(dtype, hd)):
+    if codes and not attention_prefill_supported(dtype, hd):
         _attention_kv4_direct(q, *args, cu, 0, N, B, max_len, reach, splits, dt, dev)
         return out
     n0 = 0
