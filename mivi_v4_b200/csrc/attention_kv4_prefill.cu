@@ -1,4 +1,4 @@
-// Attention of many query tokens a sequence over a cache held in 4 bits (kv4.cuh), on the fifth-generation tensor cores: bfloat16, heads of 64,
+// Attention of many query tokens a sequence over a cache held in 4 bits (kv4.cuh), on the fifth-generation tensor cores: bfloat16, heads of up to 64,
 // pages of any size, optional window.  Flash attention whose two products are tcgen05.mma in half precision with their results in tensor
 // memory; the codes become operands on their way into shared memory, so nothing of the cache is written out in between.
 //
@@ -111,11 +111,13 @@ struct Segment {
 };
 static_assert(sizeof(Segment) <= 96, "segment ring");
 
+// EXACT: the head size is 64; else it is hd_, below that, and operands' columns behind it meet zeros of the queries or are not read
+template <bool EXACT>
 __global__ void __launch_bounds__(KQ_THREADS, 1)
 attention_kv4_prefill_kernel(const __nv_bfloat16* __restrict__ q, const unsigned char* __restrict__ pool, const int* __restrict__ page_table,
                              int table_stride, int page_shift, const int* __restrict__ cu, const int* __restrict__ starts,
                              __nv_bfloat16* __restrict__ o, float* __restrict__ part_o, float* __restrict__ part_ml,
-                             int* __restrict__ tickets, int n_seqs, int nh, int nkv, float scale_log2, int window, int whole, int* __restrict__ err) {
+                             int* __restrict__ tickets, int n_seqs, int nh, int nkv, int hd_, float scale_log2, int window, int whole, int* __restrict__ err) {
     extern __shared__ unsigned char smem_raw[];
     __shared__ int scan[KQ_WARPS], is_last;
     __shared__ volatile int raising[TILES][4];                   // a warp of a half is at its exponentials
@@ -136,7 +138,7 @@ attention_kv4_prefill_kernel(const __nv_bfloat16* __restrict__ q, const unsigned
     const unsigned bar0 = smem_u32(bars);
     auto bar = [&](int i) { return bar0 + 8u * (unsigned)i; };
     const int warp = warp_index(), lane = threadIdx.x & 31, tid = threadIdx.x;
-    const int group = nh / nkv;
+    const int group = nh / nkv, hd = EXACT ? HD : hd_;
     const float per_group = 1.0f / (float)group;
 
     if (tid == 0) {
@@ -297,7 +299,7 @@ attention_kv4_prefill_kernel(const __nv_bfloat16* __restrict__ q, const unsigned
         // registers move from this warpgroup and the last to the softmax warps' (128 x 64 + 128 x 32 + 256 x 208 of the 512 x 128 at launch)
         asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
         const int page_size = 1 << page_shift, key_of = warp * 32 + lane;
-        const size_t head_bytes = kv4_head_bytes(page_size, HD);
+        const size_t head_bytes = kv4_head_bytes(page_size, hd);
         bool ok = true;
         int it = 0;
         for (int k = 0; ok; next(k), ++k) {
@@ -321,7 +323,14 @@ attention_kv4_prefill_kernel(const __nv_bfloat16* __restrict__ q, const unsigned
             auto fetch = [&](uint4 (&w)[2], int at) {
                 w[0] = w[1] = make_uint4(0u, 0u, 0u, 0u);
                 if (from != nullptr) {
-                    if (page_shift) {
+                    if (!EXACT) {                                // (a row is at 4 bytes)
+                        const unsigned* x = reinterpret_cast<const unsigned*>(from + at + row * (hd >> 1));
+                        unsigned c[8];
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) c[i] = 8 * i < hd ? x[i] : 0u;
+                        w[0] = make_uint4(c[0], c[1], c[2], c[3]);
+                        w[1] = make_uint4(c[4], c[5], c[6], c[7]);
+                    } else if (page_shift) {
                         const uint4* x = reinterpret_cast<const uint4*>(from + at + row * (HD / 2));
                         w[0] = x[0];
                         w[1] = x[1];
@@ -332,11 +341,11 @@ attention_kv4_prefill_kernel(const __nv_bfloat16* __restrict__ q, const unsigned
                     }
                 }
             };
-            auto fetch_numbers = [&]() { np = from != nullptr ? *reinterpret_cast<const uint2*>(from + page_size * HD + row * 8) : make_uint2(0u, 0u); };
+            auto fetch_numbers = [&]() { np = from != nullptr ? *reinterpret_cast<const uint2*>(from + page_size * hd + row * 8) : make_uint2(0u, 0u); };
             place_of(g.kb);
             fetch_numbers();
             fetch(kc, 0);
-            fetch(vc, page_size * (HD / 2));
+            fetch(vc, page_size * (hd >> 1));
             for (int j = 0; j < g.n; ++j, ++it) {
                 const int s = it % STAGES;
                 const unsigned ph = (unsigned)(it / STAGES) & 1u;
@@ -370,7 +379,7 @@ attention_kv4_prefill_kernel(const __nv_bfloat16* __restrict__ q, const unsigned
                 hand_over(B_KFULL);
                 if (!(ok = mbar_wait_warp(bar(B_VEMPTY + s), ph ^ 1u, err, 162))) break;
                 put(v_ptr + s * KV_BYTES, vc, p.vs, p.vz, pow2f(-ev));
-                if (j + 1 < g.n) fetch(vc, page_size * (HD / 2));
+                if (j + 1 < g.n) fetch(vc, page_size * (hd >> 1));
                 hand_over(B_VFULL);
             }
         }
@@ -485,11 +494,11 @@ attention_kv4_prefill_kernel(const __nv_bfloat16* __restrict__ q, const unsigned
             int ex = 0;
             bool fine = true;                                    // the row's elements are finite
             if (my_nb > 0) {                                     // (a half without key blocks is not waited for, and may be segments ahead)
-                const uint4* from = reinterpret_cast<const uint4*>(q + (size_t)max(row_at, 0) * HD);
+                const uint4* from = reinterpret_cast<const uint4*>(q + (size_t)max(row_at, 0) * hd);
                 uint4 raw[8];
                 float top = 0.f;
 #pragma unroll
-                for (int c = 0; c < 8; ++c) raw[c] = live ? from[c] : make_uint4(0u, 0u, 0u, 0u);
+                for (int c = 0; c < 8; ++c) raw[c] = live && (EXACT || 8 * c < hd) ? from[c] : make_uint4(0u, 0u, 0u, 0u);
 #pragma unroll
                 for (int c = 0; c < 8; ++c) {
                     const unsigned x[4] = {raw[c].x, raw[c].y, raw[c].z, raw[c].w};
@@ -677,7 +686,7 @@ attention_kv4_prefill_kernel(const __nv_bfloat16* __restrict__ q, const unsigned
                 for (int i = 0; i < 8; ++i) {
                     const int rr = 4 * i + (lane >> 3), row = __shfl_sync(0xffffffffu, row_at, rr), c = lane & 7;
                     const uint4 w = *reinterpret_cast<const uint4*>(q_rows + (quarter * 32 + rr) * 128 + ((c ^ (rr & 7)) << 4));
-                    if (row >= 0) *reinterpret_cast<uint4*>(o + (size_t)row * HD + 8 * c) = w;
+                    if (row >= 0 && (EXACT || 8 * c < hd)) *reinterpret_cast<uint4*>(o + (size_t)row * hd + 8 * c) = w;
                 }
                 __syncwarp();
             };
@@ -748,24 +757,27 @@ attention_kv4_prefill_kernel(const __nv_bfloat16* __restrict__ q, const unsigned
 
 }  // namespace
 
-// bfloat16, heads of 64.  cu and starts are those of ``n_seqs`` neighbouring sequences (cu counts from q's first row), page_table their rows; at most
+// bfloat16, heads of 8 to 64 in steps of 8.  cu and starts are those of ``n_seqs`` neighbouring sequences (cu counts from q's first row), page_table their rows; at most
 // 1,024 sequences of at least one token, and 1,024 tiles of 256 rows (a sequence's tokens times the heads of a kv head).  whole: a block a tile and
 // kv head (grid: tiles * nkv); else grid blocks, one a multiprocessor at most, share all key blocks.  part_o [2 grid, 16, 256, 4],
 // part_ml [2 grid, 256, 2] float32 and tickets [tiles * nkv] (zero) are used unless whole.
 MV_API int mv_attention_kv4_prefill(const void* q, const void* pool, const int* page_table, int table_stride, int page_size, const int* cu,
-                                    const int* starts, void* o, float* part_o, float* part_ml, int* tickets, int n_seqs, int nh, int nkv,
+                                    const int* starts, void* o, float* part_o, float* part_ml, int* tickets, int n_seqs, int nh, int nkv, int hd,
                                     float scale, int window, int whole, int grid, int* err, cudaStream_t stream) {
     if (n_seqs <= 0 || grid <= 0) return 0;
-    if (n_seqs > KQ_MOST || nkv < 1 || nh % nkv || page_size < 1 || (page_size & (page_size - 1)) ||
+    if (n_seqs > KQ_MOST || nkv < 1 || hd < 8 || hd > HD || hd % 8 || nh % nkv || page_size < 1 || (page_size & (page_size - 1)) ||
         (((uintptr_t)q | (uintptr_t)pool | (uintptr_t)o) & 15))
         return (int)cudaErrorInvalidValue;
     int page_shift = 0;
     while ((1 << page_shift) < page_size) ++page_shift;
-    const cudaError_t e = mv_allow_smem<attention_kv4_prefill_kernel>(KQ_SMEM);
-    if (e != cudaSuccess) return (int)e;
-    // a plain launch, not a programmatic one (see attention_decode_tc.cu)
-    attention_kv4_prefill_kernel<<<grid, KQ_THREADS, KQ_SMEM, stream>>>(
-        (const __nv_bfloat16*)q, (const unsigned char*)pool, page_table, table_stride, page_shift, cu, starts, (__nv_bfloat16*)o, part_o, part_ml,
-        tickets, n_seqs, nh, nkv, scale * 1.4426950408889634f, window, whole, err);
-    return mv_launch_status();
+    auto go = [&](auto kernel, cudaError_t e) {
+        if (e != cudaSuccess) return (int)e;
+        // a plain launch, not a programmatic one (see attention_decode_tc.cu)
+        kernel<<<grid, KQ_THREADS, KQ_SMEM, stream>>>((const __nv_bfloat16*)q, (const unsigned char*)pool, page_table, table_stride, page_shift, cu, starts,
+                                                      (__nv_bfloat16*)o, part_o, part_ml, tickets, n_seqs, nh, nkv, hd, scale * 1.4426950408889634f,
+                                                      window, whole, err);
+        return mv_launch_status();
+    };
+    return hd == HD ? go(attention_kv4_prefill_kernel<true>, mv_allow_smem<attention_kv4_prefill_kernel<true>>(KQ_SMEM))
+                    : go(attention_kv4_prefill_kernel<false>, mv_allow_smem<attention_kv4_prefill_kernel<false>>(KQ_SMEM));
 }

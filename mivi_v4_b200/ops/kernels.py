@@ -137,7 +137,7 @@ _SIGNATURES = {
         "mv_attention_decode_tc": [_P, _P, _Q, _P, _I, _P, _P, _P, _P, _P, _I, _I, _I, _F, _I, _P, _P],
         "mv_attention_prefill_tc": [_P, _P, _Q, _P, _I, _P, _P, _P, _I, _I, _I, _I, _F, _P, _P],
         "mv_attention_kv4_decode": [_P, _P, _P, _I, _I, _P, _P, _P, _I, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _F, _I, _I, _I, _I, _I, _I, _I, _I, _P, _P],
-        "mv_attention_kv4_prefill": [_P, _P, _P, _I, _I, _P, _P, _P, _P, _P, _P, _I, _I, _I, _F, _I, _I, _I, _P, _P],
+        "mv_attention_kv4_prefill": [_P, _P, _P, _I, _I, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _F, _I, _I, _I, _P, _P],
         "mv_latent_attention_decode": [_P, _P, _Q, _P, _I, _I, _P, _P, _P, _P, _I, _I, _I, _I, _F, _I, _I, _P, _P, _P, _P],
         "mv_latent_query": [_P, _I, _I, _P, _P, _P, _I, _I, _I, _I, _I, _F, _P],
         "mv_latent_gather": [_P, _Q, _P, _I, _I, _P, _P, _I, _I, _I, _I, _P, _P, _I, _P],
@@ -2752,22 +2752,17 @@ def kv4_read(pool: torch.Tensor, page_table, positions, seq_of, k_out: torch.Ten
 # Tokens a sequence up to which a step's queries read the codes themselves, in a kernel made for few.  Heads of 64, 32 / 8 of them: 16 sequences
 # of 6 tokens behind 3,000 take 29 us there and 51 us in the tcgen05 kernel, 8 of 9 behind 2,000 22 and 31, 8 of 20 39 and 31.
 KV4_DIRECT_TOKENS = 16
-# Where many tokens have their cache read back first, these few do better without it behind a long context: at most so many in the step,
-# each behind at least so many keys (``attention_kv4``).
-KV4_FAR_TOKENS, KV4_FAR_KEYS = 256, 32
 KV4_READ_BYTES = 1 << 30            # most of the cache that is read back at a time, unless one sequence alone is more
 
 
-def kv4_runs(starts, lens, window: int, page_size: int, page_bytes: int, far: bool = False):
+def kv4_runs(starts, lens, window: int, page_size: int, page_bytes: int):
     """How a step's sequences are attended to: [(first sequence, one past the last, pages to read back, 0 for none)].  Neighbours
     that bring at most ``KV4_DIRECT_TOKENS`` tokens each read the codes themselves, together; the others' pages (``page_bytes``
-    each once they are read back) are read back first, for as many neighbours together as ``KV4_READ_BYTES`` holds.  ``far``: so do the
-    sequences of a step of at most ``KV4_FAR_TOKENS`` tokens that see ``KV4_FAR_KEYS`` cached keys for each that they bring."""
-    far = far and sum(lens) <= KV4_FAR_TOKENS
+    each once they are read back) are read back first, for as many neighbours together as ``KV4_READ_BYTES`` holds."""
     runs = []
     for b, (s, n) in enumerate(zip(starts, lens)):
         pages = 0
-        if n > KV4_DIRECT_TOKENS and not (far and (min(s, window) if window > 0 else s) >= KV4_FAR_KEYS * n):
+        if n > KV4_DIRECT_TOKENS:
             first = max(0, s - window + 1) // page_size if window > 0 else 0
             pages = -(-(s + n) // page_size) - first
         if runs and (runs[-1][2] > 0) == (pages > 0) and (runs[-1][2] + pages) * page_bytes <= KV4_READ_BYTES:
@@ -2827,20 +2822,18 @@ def attention_kv4(q: torch.Tensor, pool: torch.Tensor, page_table, positions, se
                               reach, splits, dt, dev)
         return out
     args = (pool, page_table, W, page_size, positions, seq_of, starts, out, nh, nkv, hd, scale, window, ws)
-    fused = attention_kv4_prefill_supported(dtype, hd)
-    codes = not fused and attention_kv4_decode_supported(dtype, page_size)
-    # (head sizes that no tensor-core kernel of many tokens takes, 8 / 2 heads of 256: 2,048 tokens of a prompt take 296 us over the codes in
-    # launches of 256 rows, 3,840 us read back)
-    if codes and not attention_prefill_supported(dtype, hd):
+    fused = attention_kv4_prefill_supported(dtype, hd) and max_len * (nh // nkv) <= 256 * KV4_PREFILL_MOST
+    # Larger heads stay with the codes, too: rows read back in bfloat16 would be off by as much again as the result's own rounding, and take the
+    # memory that 4 bits save.  2,048 tokens of a prompt, 16 / 4 heads of 128: 186 us so, 127 us read back; 64 tokens behind 8,000: 51 and 240;
+    # 8 / 2 heads of 256, which no tensor-core kernel of many tokens takes once they are read back: 296 us and 3,840 us.
+    if not fused and attention_kv4_decode_supported(dtype, page_size):
         _attention_kv4_direct(q, *args, cu, 0, N, B, max_len, reach, splits, dt, dev)
         return out
     n0 = 0
-    # (far: heads of 128, 16 / 4 of them, 20 tokens behind 8,000: 30 us over the codes, 240 us read back; 64: 51 and 240)
-    for b0, b1, pages in kv4_runs(host_starts, host_lens, window, page_size, 0 if fused else 2 * nkv * page_size * hd * q.element_size(),
-                                  codes):
+    for b0, b1, pages in kv4_runs(host_starts, host_lens, window, page_size, 0 if fused else 2 * nkv * page_size * hd * q.element_size()):
         n1 = n0 + sum(host_lens[b0:b1])
         if pages and fused:
-            _attention_kv4_prefill(q, pool, page_table, W, page_size, cu, starts, out, nh, nkv, scale, window, ws, b0, b1, host_starts, host_lens, dev)
+            _attention_kv4_prefill(q, pool, page_table, W, page_size, cu, starts, out, nh, nkv, hd, scale, window, ws, b0, b1, host_starts, host_lens, dev)
         elif pages == 0:
             _attention_kv4_direct(q, *args, cu, n0, n1, b1 - b0, max(host_lens[b0:b1]), reach, splits, dt, dev)
         else:
@@ -2935,8 +2928,8 @@ def _attention_kv4_direct(q, pool, page_table, W, page_size, positions, seq_of, 
 
 
 def attention_kv4_prefill_supported(dtype: torch.dtype, hd: int) -> bool:
-    """What the tcgen05 kernel over the codes takes: bfloat16 and heads of 64 (pages of any size, windows)."""
-    return dtype == torch.bfloat16 and hd == 64
+    """What the tcgen05 kernel over the codes takes: bfloat16 and heads of up to 64 (pages of any size, windows)."""
+    return dtype == torch.bfloat16 and hd <= 64
 
 
 KV4_PREFILL_MOST = 1024             # most sequences, and most tiles of 256 rows, of a launch (attention_kv4_prefill.cu)
@@ -2945,7 +2938,7 @@ KV4_PREFILL_MOST = 1024             # most sequences, and most tiles of 256 rows
 @functools.lru_cache(maxsize=256)
 def attention_kv4_prefill_plan(starts: tuple, lens: tuple, group: int, nkv: int, window: int):
     """[(sequences, tiles, whether a block takes whole tiles and kv heads, blocks)] for the launches over neighbouring sequences that bring
-    ``lens`` tokens from ``starts`` on.  A tile is 256 rows, tokens by the heads of a kv head.  Costs are counted in key blocks of 128, 2 us
+    ``lens`` tokens from ``starts`` on, none of them more than a launch takes.  A tile is 256 rows, tokens by the heads of a kv head.  Costs are counted in key blocks of 128, 2 us
     each: a whole tile's beginning and end take about one and a half more, a tile that is shared among blocks about five for each of them
     (its parts are written, fetched and put together).  The way that ends earlier is taken."""
     plan, b, sms = [], 0, n_sms()
@@ -2959,9 +2952,6 @@ def attention_kv4_prefill_plan(starts: tuple, lens: tuple, group: int, nkv: int,
                 last, first = starts[end] + (min(rows, r + 256) - 1) // group, starts[end] + r // group
                 sizes.append(last // 128 + 1 - (max(0, first - window + 1) // 128 if window > 0 else 0))
             end += 1
-        if end == b:
-            raise KernelError(f"attention_kv4: {lens[b]} tokens of one sequence by {group} heads a kv head in one step; at most "
-                              f"{KV4_PREFILL_MOST * 256} rows")
         units, total = len(sizes) * nkv, sum(sizes) * nkv
         blocks = min(sms, units)
         busy = [0.0] * blocks
@@ -2976,7 +2966,7 @@ def attention_kv4_prefill_plan(starts: tuple, lens: tuple, group: int, nkv: int,
     return plan
 
 
-def _attention_kv4_prefill(q, pool, page_table, W, page_size, cu, starts, out, nh, nkv, scale, window, ws, b0, b1, host_starts, host_lens, dev):
+def _attention_kv4_prefill(q, pool, page_table, W, page_size, cu, starts, out, nh, nkv, hd, scale, window, ws, b0, b1, host_starts, host_lens, dev):
     """Sequences b0 .. b1 - 1, many tokens each, over the codes on tcgen05."""
     flag = _error_flags.get(dev)
     for n_seqs, tiles, whole, grid in attention_kv4_prefill_plan(tuple(host_starts[b0:b1]), tuple(host_lens[b0:b1]), nh // nkv, nkv, window):
@@ -2988,18 +2978,19 @@ def _attention_kv4_prefill(q, pool, page_table, W, page_size, cu, starts, out, n
             _guard("bf16", "attention_kv4_prefill", q.device, n_pages=pool.shape[0])
         _check(_fn("bf16", "mv_attention_kv4_prefill")(
             q.data_ptr(), pool.data_ptr(), page_table.data_ptr() + 4 * W * b0, W, page_size, cu.data_ptr() + 4 * b0, starts.data_ptr() + 4 * b0,
-            out.data_ptr(), parts, None if whole else parts + 2 * grid * 256 * 64 * 4, tickets, n_seqs, nh, nkv, scale, window, whole, grid,
+            out.data_ptr(), parts, None if whole else parts + 2 * grid * 256 * 64 * 4, tickets, n_seqs, nh, nkv, hd, scale, window, whole, grid,
             (_error_flag(q.device) if flag is None else flag).data_ptr(), _stream()), "mv_attention_kv4_prefill")
         b0 += n_seqs
 
 
 def _attention_kv4_pages(q, pool, page_table, W, page_size, positions, seq_of, starts, out, nh, nkv, hd, scale, window, ws, cu, b0, b1, n0, n1, pages,
                          host_lens):
-    """Sequences b0 .. b1 - 1: their pages are read back into a pool of their own, which the attention kernels of many tokens read."""
+    """Sequences b0 .. b1 - 1: their pages are read back into a pool of their own, which the attention kernels of many tokens read
+    (float32, and pages of fewer than 16 tokens)."""
     n_seqs = b1 - b0
     if n_seqs > 65535 or nkv > 65535:
         raise KernelError(f"attention_kv4: {n_seqs} sequences and {nkv} kv heads in one launch; each may be 65535 at most")
-    # (a power of two pages: the pool keeps its shape, and with it its tensor map, as sequences grow)
+    # (a power of two pages: the pool keeps its shape as sequences grow)
     read = ws.get("kv4_pages", (1 << (pages - 1).bit_length(), 2, nkv, page_size, hd), q.dtype)
     table = ws.get("kv4_table", (page_table.shape[0], W), torch.int32)
     cu_run, starts_run, table_run = cu[b0:b1 + 1], starts[b0:b1], table[b0:b1]
@@ -3008,9 +2999,7 @@ def _attention_kv4_pages(q, pool, page_table, W, page_size, positions, seq_of, s
         pool.data_ptr(), page_table.data_ptr() + 4 * W * b0, W, page_size, cu_run.data_ptr(), starts_run.data_ptr(), window,
         read.data_ptr(), _dt(read), table_run.data_ptr(), W, n_seqs, nkv, hd, _stream()), "mv_kv4_read_pages")
     account(pages * nkv * page_size * (hd + 8 + 2 * hd * read.element_size()))
-    if n1 - n0 >= 128 * n_seqs and attention_prefill_tc_supported(q.dtype, hd, read, window):
-        attention_prefill_tc(q, read, table_run, cu_run, starts_run, out, n_seqs, nh, nkv, hd, scale)
-    elif attention_prefill_supported(q.dtype, hd):
+    if attention_prefill_supported(q.dtype, hd):
         attention_prefill(q, read, table_run, cu_run, starts_run, out, n_seqs, nh, nkv, hd, scale, window)
     else:
         attention_generic(q[n0:n1], read, table, positions[n0:n1], seq_of[n0:n1], out[n0:n1], nh, nkv, hd, scale, window,

@@ -65,6 +65,32 @@ def test_both_ways_to_share_the_work(monkeypatch, way, nh, nkv, page, window, le
         assert torch.equal(out, attend_all(q, dev_pool, rows, lengths, lens, nh, nkv, 64, page, window, ws))
 
 
+@pytest.mark.parametrize("whole", [True, False])
+@pytest.mark.parametrize("nh,nkv,hd,page,window", [(8, 2, 48, 64, 0), (3, 1, 8, 1, 0), (4, 4, 16, 2, 70), (6, 2, 40, 16, 0), (5, 1, 56, 1, 100), (16, 8, 32, 64, 0),
+                                                   (24, 1, 24, 128, 0)])
+def test_smaller_heads(monkeypatch, whole, nh, nkv, hd, page, window):
+    lens, before = [20, 300, 150], [500, 0, 77]
+    lengths = [a + m for a, m in zip(before, lens)]
+    rows, total = tables(lengths, page, seed=hd)
+    pool, rk, rv = filled(total, nkv, page, hd, seed=nh + hd)
+    q = torch.randn(sum(lens), nh, hd, generator=torch.Generator().manual_seed(9)).bfloat16()
+    plan = K().attention_kv4_prefill_plan
+    monkeypatch.setattr(K(), "attention_kv4_prefill_plan", lambda *a: [(n, tiles, whole, min(148, tiles * nkv) if whole else 13) for n, tiles, _, _ in plan(*a)])
+    out = attend_all(q, pool.to(DEV), rows, lengths, lens, nh, nkv, hd, page, window)
+    held_to_half(out, q, rk, rv, rows, lengths, lens, page, window, some(lens))
+
+
+def test_a_run_of_more_rows_than_the_tables_hold(monkeypatch):
+    """Such a step takes the other kernels."""
+    nh, nkv, hd, page, lens, lengths = 8, 1, 64, 64, [130], [130]
+    monkeypatch.setattr(K(), "KV4_PREFILL_MOST", 4)
+    monkeypatch.setattr(K(), "_attention_kv4_prefill", None)
+    rows, total = tables(lengths, page, seed=hd)
+    pool, rk, rv = filled(total, nkv, page, hd, seed=nh + hd)
+    q = torch.randn(130, nh, hd, generator=torch.Generator().manual_seed(9)).bfloat16()
+    check(attend_all(q, pool.to(DEV), rows, lengths, lens, nh, nkv, hd, page, 0), q, rk, rv, rows, lengths, lens, page, 0, torch.bfloat16)
+
+
 def test_more_sequences_than_a_launch_takes():
     nh, nkv, page, n_seqs = 2, 1, 16, 1100
     lens = [17 + b % 3 for b in range(n_seqs)]
@@ -79,8 +105,9 @@ def test_more_sequences_than_a_launch_takes():
 
 @pytest.mark.parametrize("nh,nkv,hd,page,window", [(4, 1, 72, 16, 0), (2, 2, 256, 64, 0), (12, 2, 40, 64, 100), (6, 1, 24, 32, 0)])
 @pytest.mark.parametrize("lens,before", [([600], [3]), ([7, 255, 1, 300], [10, 5, 0, 64]), ([3] * 120, [1] * 120)])
-def test_more_rows_than_a_launch_takes(nh, nkv, hd, page, window, lens, before):
-    """Launches begin and end within runs, and within what one block takes of a run."""
+def test_more_rows_than_a_launch_takes(monkeypatch, nh, nkv, hd, page, window, lens, before):
+    """Launches of the kernel for few tokens begin and end within runs, and within what one block takes of a run."""
+    monkeypatch.setattr(K(), "attention_kv4_prefill_supported", lambda dtype, hd: False)
     lengths = [a + m for a, m in zip(before, lens)]
     rows, total = tables(lengths, page, seed=hd)
     pool, rk, rv = filled(total, nkv, page, hd, seed=hd + 1)
@@ -96,14 +123,14 @@ def test_more_rows_than_a_launch_takes(nh, nkv, hd, page, window, lens, before):
 
 @pytest.mark.parametrize("lens,before", [([40], [1280]), ([17, 60, 2], [544, 1920, 0]), ([40], [1279]), ([20, 200, 30], [700, 100, 1000])])
 def test_short_runs_behind_long_contexts(lens, before):
-    """Heads of 128: over the codes, read back, and both in one step."""
+    """Heads of 128: more rows than a launch takes, and fewer."""
     nh, nkv, hd, page = 4, 2, 128, 64
     lengths = [a + m for a, m in zip(before, lens)]
     rows, total = tables(lengths, page, seed=5)
     pool, rk, rv = filled(total, nkv, page, hd, seed=6)
     q = torch.randn(sum(lens), nh, hd, generator=torch.Generator().manual_seed(8)).bfloat16()
     out = attend_all(q, pool.to(DEV), rows, lengths, lens, nh, nkv, hd, page, 0)
-    check(out, q, rk, rv, rows, lengths, lens, page, 0, torch.bfloat16)
+    check(out, q, rk, rv, rows, lengths, lens, page, 0, torch.bfloat16, pages=False)
 
 
 def test_recorded_prompts_and_two_recordings_of_one_workspace():
