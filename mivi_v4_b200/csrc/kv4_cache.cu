@@ -525,14 +525,14 @@ attention_kv4_kernel(const T* __restrict__ q, const unsigned char* __restrict__ 
             for (int h = 0; h < GT; ++h) dot[h] = 0.f;
             for (int w = 0; w < words; ++w) {
                 float c[8];
-                kv4_unpack8(kc[w], 1.f, 0.f, c);
+                kv4_unpack8(kc[w], 1.f, -8.f, c);
 #pragma unroll
                 for (int h = 0; h < GT; ++h)
 #pragma unroll
                     for (int e = 0; e < 8; ++e) dot[h] = fmaf(c[e], qs[h * hd + 8 * w + e], dot[h]);
             }
 #pragma unroll
-            for (int h = 0; h < GT; ++h) s[h] = fmaf(p.ks, dot[h], p.kz * qsum[h]);
+            for (int h = 0; h < GT; ++h) s[h] = fmaf(p.ks, dot[h], fmaf(8.f, p.ks, p.kz) * qsum[h]);       // (codes less 8: little cancels)
         }
 #pragma unroll
         for (int h = 0; h < GT; ++h) {

@@ -2752,17 +2752,20 @@ def kv4_read(pool: torch.Tensor, page_table, positions, seq_of, k_out: torch.Ten
 # Tokens a sequence up to which a step's queries read the codes themselves, in a kernel made for few.  Heads of 64, 32 / 8 of them: 16 sequences
 # of 6 tokens behind 3,000 take 29 us there and 51 us in the tcgen05 kernel, 8 of 9 behind 2,000 22 and 31, 8 of 20 39 and 31.
 KV4_DIRECT_TOKENS = 16
+# The same where more tokens have their cache read back (float32, and pages of fewer than 16 tokens): 32 / 8 heads of 64 in float32, 64 tokens behind
+# 2,000 take 124 us over the codes and 393 us read back, 512 of a prompt 147 and 97 us, 1,500 1,120 and 480 us; 3 / 1 heads of 96 280 and 337 us.
+KV4_DIRECT_INSTEAD = 256
 KV4_READ_BYTES = 1 << 30            # most of the cache that is read back at a time, unless one sequence alone is more
 
 
-def kv4_runs(starts, lens, window: int, page_size: int, page_bytes: int):
+def kv4_runs(starts, lens, window: int, page_size: int, page_bytes: int, few: int = KV4_DIRECT_TOKENS):
     """How a step's sequences are attended to: [(first sequence, one past the last, pages to read back, 0 for none)].  Neighbours
-    that bring at most ``KV4_DIRECT_TOKENS`` tokens each read the codes themselves, together; the others' pages (``page_bytes``
+    that bring at most ``few`` tokens each read the codes themselves, together; the others' pages (``page_bytes``
     each once they are read back) are read back first, for as many neighbours together as ``KV4_READ_BYTES`` holds."""
     runs = []
     for b, (s, n) in enumerate(zip(starts, lens)):
         pages = 0
-        if n > KV4_DIRECT_TOKENS:
+        if n > few:
             first = max(0, s - window + 1) // page_size if window > 0 else 0
             pages = -(-(s + n) // page_size) - first
         if runs and (runs[-1][2] > 0) == (pages > 0) and (runs[-1][2] + pages) * page_bytes <= KV4_READ_BYTES:
@@ -2823,14 +2826,15 @@ def attention_kv4(q: torch.Tensor, pool: torch.Tensor, page_table, positions, se
         return out
     args = (pool, page_table, W, page_size, positions, seq_of, starts, out, nh, nkv, hd, scale, window, ws)
     fused = attention_kv4_prefill_supported(dtype, hd) and max_len * (nh // nkv) <= 256 * KV4_PREFILL_MOST
-    # Larger heads stay with the codes, too: rows read back in bfloat16 would be off by as much again as the result's own rounding, and take the
-    # memory that 4 bits save.  2,048 tokens of a prompt, 16 / 4 heads of 128: 186 us so, 127 us read back; 64 tokens behind 8,000: 51 and 240;
-    # 8 / 2 heads of 256, which no tensor-core kernel of many tokens takes once they are read back: 296 us and 3,840 us.
-    if not fused and attention_kv4_decode_supported(dtype, page_size):
+    # Larger heads in bfloat16 stay with the codes, too: rows read back would be off by as much again as the result's own rounding, and take the
+    # memory that 4 bits save.  2,048 tokens of a prompt, 16 / 4 heads of 128: 186 us so, 127 us read back; 64 tokens behind 8,000: 51 and 240.
+    # And so do head sizes that no kernel of many tokens takes in tiles: 8 / 2 heads of 256, 2,048 tokens: 296 us so, 3,840 us read back.
+    few = KV4_DIRECT_TOKENS if fused else KV4_DIRECT_INSTEAD
+    if not fused and (max_len <= few or hd > 128 or attention_kv4_decode_supported(dtype, page_size)):
         _attention_kv4_direct(q, *args, cu, 0, N, B, max_len, reach, splits, dt, dev)
         return out
     n0 = 0
-    for b0, b1, pages in kv4_runs(host_starts, host_lens, window, page_size, 0 if fused else 2 * nkv * page_size * hd * q.element_size()):
+    for b0, b1, pages in kv4_runs(host_starts, host_lens, window, page_size, 0 if fused else 2 * nkv * page_size * hd * q.element_size(), few):
         n1 = n0 + sum(host_lens[b0:b1])
         if pages and fused:
             _attention_kv4_prefill(q, pool, page_table, W, page_size, cu, starts, out, nh, nkv, hd, scale, window, ws, b0, b1, host_starts, host_lens, dev)

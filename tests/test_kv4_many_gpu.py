@@ -181,3 +181,16 @@ def test_rows_of_any_size(qs, ks, vs):
     q = (torch.randn(m, nh, 64, generator=g).clamp(-2, 2) * qs).bfloat16()
     out = attend_all(q, pool.to(DEV), [[3, 0, 1, 4, 2]], [300], [m], nh, nkv, 64, page, 0)
     held_to_half(out, q, rk, rv, [[3, 0, 1, 4, 2]], [300], [m], page, 0, some([m], 19))
+
+
+@pytest.mark.parametrize("dtype,nh,nkv,hd,page,window", [(torch.float32, 4, 2, 64, 64, 0), (torch.float32, 3, 1, 96, 8, 90), (torch.float32, 2, 1, 256, 16, 0),
+                                                         (torch.bfloat16, 4, 2, 96, 8, 0), (torch.bfloat16, 2, 2, 80, 1, 40)])
+@pytest.mark.parametrize("lens,before", [([256, 3, 257], [70, 0, 10]), ([300], [0]), ([30, 200, 90], [3, 500, 0])])
+def test_float32_and_small_pages(dtype, nh, nkv, hd, page, window, lens, before):
+    """Over the codes, read back, and both in one step."""
+    lengths = [a + m for a, m in zip(before, lens)]
+    rows, total = tables(lengths, page, seed=hd)
+    pool, rk, rv = filled(total, nkv, page, hd, seed=hd + 2)
+    q = torch.randn(sum(lens), nh, hd, generator=torch.Generator().manual_seed(8)).to(dtype)
+    out = attend_all(q, pool.to(DEV), rows, lengths, lens, nh, nkv, hd, page, window)
+    check(out, q, rk, rv, rows, lengths, lens, page, window, dtype, pages=max(lens) > K().KV4_DIRECT_INSTEAD)
