@@ -45,15 +45,16 @@ constexpr int BQ = 128, TILES = 2, ROWS = BQ * TILES, BKV = 128, HD = 64;
 constexpr int Q_BYTES = BQ * HD * 2, KV_BYTES = BKV * HD * 2, P_BYTES = BQ * BKV * 2;
 constexpr int STAGES = 3, EXPS = 8, KQ_MOST = 1024;              // most sequences, and most tiles, of a launch
 constexpr int KQ_EXTRA = 3;                                      // key blocks that a tile's beginning and end count for
-constexpr int KQ_BARS = TILES * Q_BYTES + 2 * STAGES * KV_BYTES + TILES * P_BYTES, KQ_EXPS = KQ_BARS + 256, KQ_SEGS = KQ_EXPS + EXPS * 32, KQ_TABLES = KQ_SEGS + 4 * 96,
+constexpr int KQ_BARS = TILES * Q_BYTES + 2 * STAGES * KV_BYTES + TILES * P_BYTES, KQ_EXPS = KQ_BARS + 272, KQ_SEGS = KQ_EXPS + EXPS * 32, KQ_TABLES = KQ_SEGS + 4 * 96,
               KQ_SMEM = KQ_TABLES + (3 * KQ_MOST + 4) * 4 + 1024;
 static_assert(KQ_SMEM <= 227 * 1024 - 512, "shared memory");
 constexpr unsigned S_COL0 = 0, O_COL0 = 256;                     // of half t: S 128 t on, O 64 t on
 constexpr float RESCALE_ABOVE = 8.0f;
 
 enum { B_Q = 0, B_KFULL = B_Q + TILES, B_KEMPTY = B_KFULL + STAGES, B_VFULL = B_KEMPTY + STAGES, B_VEMPTY = B_VFULL + STAGES,
-       B_SFULL = B_VEMPTY + STAGES, B_PFULL = B_SFULL + TILES, B_PVDONE = B_PFULL + TILES, B_SFREE = B_PVDONE + TILES, B_SEGFULL = B_SFREE + TILES, B_SEGEMPTY = B_SEGFULL + 4, B_COUNT = B_SEGEMPTY + 4 };
-static_assert(B_COUNT * 8 + 8 <= 256, "barrier area");
+       B_SFULL = B_VEMPTY + STAGES, B_PFULL = B_SFULL + TILES, B_PVDONE = B_PFULL + TILES, B_SFREE = B_PVDONE + TILES, B_SEGFULL = B_SFREE + TILES, B_SEGEMPTY = B_SEGFULL + 4,
+       B_PARTS = B_SEGEMPTY + 4, B_LAST, B_COUNT };
+static_assert(B_COUNT * 8 + 8 <= 272, "barrier area");
 
 // MN-major operand (values: rows are keys, 128 bytes = 64 elements a row), 128-byte swizzle: 8-row groups 1024 bytes apart
 __device__ __forceinline__ unsigned long long smem_desc_mn(unsigned addr) {
@@ -159,6 +160,8 @@ attention_kv4_prefill_kernel(const __nv_bfloat16* __restrict__ q, const unsigned
             mbar_init(bar(B_SEGFULL + k), 1);
             mbar_init(bar(B_SEGEMPTY + k), 13);
         }
+        mbar_init(bar(B_PARTS), 8);
+        mbar_init(bar(B_LAST), 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == MMA_WARP) {
@@ -478,11 +481,12 @@ attention_kv4_prefill_kernel(const __nv_bfloat16* __restrict__ q, const unsigned
         unsigned char* p_row = p_ptr + t * P_BYTES + r * 128;
         unsigned char* q_rows = smem + t * Q_BYTES;
         bool ok = true;
-        int it = 0, done = 0;
+        int it = 0, done = 0, merges = 0;
         for (int k = 0;; next(k), ++k) {
             const Segment* sg = segment_at(k);
             if (sg == nullptr) break;
             const int my_nb = sg->nb[t], parts = sg->parts;
+            if (!ok) break;                                      // (a wait ran out: the others' do, too)
             const bool live = t * BQ + r < sg->nq;
             int pos = -1, row_at = -1;                           // the row's position; its place among the rows of q and o
             if (live) {
@@ -534,7 +538,7 @@ attention_kv4_prefill_kernel(const __nv_bfloat16* __restrict__ q, const unsigned
             float m = -INFINITY, l = fine ? 0.f : NAN;           // m: the row's reference, log2 units
             int ev = -126;                                       // the accumulator's power of two
             for (int j = 0; j < my_nb && ok; ++j) {
-                ok = mbar_wait(bar(B_SFULL + t), (unsigned)(done + j) & 1u, err, 169);
+                ok = mbar_wait_warp(bar(B_SFULL + t), (unsigned)(done + j) & 1u, err, 169);
                 if (!ok) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 unsigned s[4][32];
@@ -583,7 +587,7 @@ attention_kv4_prefill_kernel(const __nv_bfloat16* __restrict__ q, const unsigned
                 ev = ev_new;
                 // P (shared memory) and O (tensor memory) are the key block before's until its product is done
                 if (j > 0) {
-                    ok = mbar_wait(bar(B_PVDONE + t), (unsigned)(done + j - 1) & 1u, err, 170);
+                    ok = mbar_wait_warp(bar(B_PVDONE + t), (unsigned)(done + j - 1) & 1u, err, 170);
                     if (!ok) break;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 }
@@ -645,8 +649,9 @@ attention_kv4_prefill_kernel(const __nv_bfloat16* __restrict__ q, const unsigned
                 __syncwarp();
                 if (lane == 0) mbar_arrive(bar(B_PFULL + t));
             }
-            if (ok && my_nb > 0) ok = mbar_wait(bar(B_PVDONE + t), (unsigned)(done + my_nb - 1) & 1u, err, 171);
+            if (ok && my_nb > 0) ok = mbar_wait_warp(bar(B_PVDONE + t), (unsigned)(done + my_nb - 1) & 1u, err, 171);
             if (ok && my_nb > 0) asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            if (!ok) break;
             // ---- the rows out, by the queries' place in shared memory (a warp's own rows: whole lines leave), or a part of them
             const bool read = ok && my_nb > 0;
             const float up = pow2f(ev) * (parts == 1 ? 1.0f / l : 1.0f);
@@ -694,14 +699,21 @@ attention_kv4_prefill_kernel(const __nv_bfloat16* __restrict__ q, const unsigned
                 if (my_nb > 0) rows_out();
             } else {
                 if (live) *reinterpret_cast<float2*>(part_ml + ((size_t)slot * ROWS + t * BQ + r) * 2) = make_float2(m, l);
-                asm volatile("bar.sync 1, 256;" ::: "memory");
-                if (warp == 4 && lane == 0) {
-                    __threadfence();
-                    is_last = atomicAdd(tickets + sg->unit, 1) == parts - 1;
-                    if (is_last) tickets[sg->unit] = 0;
-                    __threadfence();
+                // (is_last changes when all eight warps have come here again, so after they have read it)
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar(B_PARTS));
+                if (warp == 4) {
+                    if (!mbar_wait_warp(bar(B_PARTS), (unsigned)merges & 1u, err, 172)) break;
+                    if (lane == 0) {
+                        __threadfence();
+                        is_last = atomicAdd(tickets + sg->unit, 1) == parts - 1;
+                        if (is_last) tickets[sg->unit] = 0;
+                        __threadfence();
+                        mbar_arrive(bar(B_LAST));
+                    }
                 }
-                asm volatile("bar.sync 1, 256;" ::: "memory");
+                if (!mbar_wait_warp(bar(B_LAST), (unsigned)merges & 1u, err, 173)) break;
+                ++merges;
                 const bool last = is_last;
                 if (last && t * BQ < sg->nq) {
                     // A part: reference (log2 units), sum, weighted values.  Where nothing was seen the sum is 0 and the part counts nothing;
@@ -738,7 +750,6 @@ attention_kv4_prefill_kernel(const __nv_bfloat16* __restrict__ q, const unsigned
                     }
                     rows_out();
                 }
-                asm volatile("bar.sync 1, 256;" ::: "memory");        // (is_last may change from here on)
             }
             it += sg->n;
             done += my_nb;

@@ -2049,7 +2049,7 @@ _error_mirrors = {}
 _ERROR_CODES = (((1, 3), "gemm_tc.cu"), ((5, 5), "gemm_tc.cu"), ((11, 21), "attention_prefill_tc.cu"), ((30, 40), "attention_decode_tc.cu"),
                 ((45, 45), "latent_attention_decode.cu"), ((51, 63), "latent_attention_tc.cu"), ((71, 76), "gemm_f32_tc.cu"),
                 ((81, 93), "attention_sink_tc.cu"), ((101, 103), "gemm_tc_swap.cu"), ((111, 115), "gemm_tc_pair.cu"),
-                ((150, 151), "attention_kv4_decode.cu"), ((160, 171), "attention_kv4_prefill.cu"))
+                ((150, 151), "attention_kv4_decode.cu"), ((160, 173), "attention_kv4_prefill.cu"))
 # the products' roles, by the last digit
 _ERROR_ROLES = {1: "the TMA producer", 2: "the MMA issuer", 3: "the epilogue", 5: "the MMA issuer (for the epilogue)"}
 
