@@ -611,10 +611,19 @@ int kd_launch(dim3 grid, cudaStream_t stream, A... args) {
 // only where heads is the whole group).  The keys are cut into pieces of ``piece`` tiles of 64 (0: such that there are about ``blocks``
 // pieces in all); ``grid`` bounds the pieces times kv heads and head tiles: blocks + N * nkv * head_tiles where piece is 0.
 // part_o [grid, 4 nt, hd] and part_ml [grid, 4 nt, 2] float32, tickets [N, nkv * head_tiles] (zero).
-MV_API int mv_attention_kv4_decode(const void* q, const void* pool, const int* page_table, int table_stride, int page_size,
-                                   const int* positions, const int* seq_of, const int* cu, int n0, const int* starts, void* o,
-                                   float* part_o, float* part_ml, int* tickets, int N, int tiles, int nh, int nkv, int hd, float scale, int window, int nt, int head_tiles, int heads,
-                                   int tokens_per_tile, int piece, int blocks, int grid, int* err, cudaStream_t stream) {
+struct AttentionKv4DecodeArgs {
+    const void *q, *pool;
+    const int *page_table, *positions, *seq_of, *cu, *starts;
+    void* o;
+    float *part_o, *part_ml;
+    int *tickets, *err;
+    cudaStream_t stream;
+    int table_stride, page_size, n0, N, tiles, nh, nkv, hd, window, nt, head_tiles, heads, tokens_per_tile, piece, blocks, grid;
+    float scale;
+};
+MV_API int mv_attention_kv4_decode(const void* record) {
+    const auto& [q, pool, page_table, positions, seq_of, cu, starts, o, part_o, part_ml, tickets, err, stream, table_stride, page_size, n0, N, tiles, nh, nkv, hd,
+                window, nt, head_tiles, heads, tokens_per_tile, piece, blocks, grid, scale] = *static_cast<const AttentionKv4DecodeArgs*>(record);
     if (N <= 0) return 0;
     if (hd % 8 || hd < 8 || hd > KV4_MAX_HEAD_DIM || nkv < 1 || nh % nkv || page_size < 16 || (page_size & (page_size - 1)) || blocks < 1 ||
         grid < 1 || piece < 0 || heads < 1 || heads * head_tiles < nh / nkv || tokens_per_tile < 1 ||

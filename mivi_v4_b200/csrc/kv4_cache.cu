@@ -312,9 +312,17 @@ kv4_prepare_kernel(const float* __restrict__ qkv, const float* __restrict__ wq, 
 }
 
 // qkv float32 [N, (nh + 2 nkv) * hd]; pool [pages, nkv, page_size * (hd + 8)] bytes.  q_out [N, nh * hd] in q_dtype.  Everything on 16 bytes.
-MV_API int mv_kv4_prepare(const float* qkv, const float* wq, const float* wk, float eps, const float* inv_freq, int half_split,
-                          const int* positions, const int* seq_of, const int* page_table, int table_stride, int page_size,
-                          void* pool, void* q_out, int q_dtype, int N, int nh, int nkv, int hd, cudaStream_t stream) {
+struct Kv4PrepareArgs {
+    const float *qkv, *wq, *wk, *inv_freq;
+    const int *positions, *seq_of, *page_table;
+    void *pool, *q_out;
+    cudaStream_t stream;
+    int half_split, table_stride, page_size, q_dtype, N, nh, nkv, hd;
+    float eps;
+};
+MV_API int mv_kv4_prepare(const void* record) {
+    const auto& [qkv, wq, wk, inv_freq, positions, seq_of, page_table, pool, q_out, stream, half_split, table_stride, page_size, q_dtype, N, nh, nkv, hd,
+                eps] = *static_cast<const Kv4PrepareArgs*>(record);
     if (N <= 0) return 0;
     if (hd % 8 || hd < 8 || hd > KV4_MAX_HEAD_DIM || page_size < 1 || (page_size & (page_size - 1)) || nkv < 1 ||
         (((uintptr_t)qkv | (uintptr_t)wq | (uintptr_t)wk | (uintptr_t)q_out | (uintptr_t)pool) & 15))
@@ -373,8 +381,16 @@ kv4_read_kernel(const unsigned char* __restrict__ pool, const int* __restrict__ 
     kv4_store8((kv ? v_out : k_out) + ((size_t)n * nkv + g) * hd + 8 * w, v);
 }
 
-MV_API int mv_kv4_read(const void* pool, const int* page_table, int table_stride, int page_size, const int* positions,
-                       const int* seq_of, void* k_out, void* v_out, int dtype, int N, int nkv, int hd, cudaStream_t stream) {
+struct Kv4ReadArgs {
+    const void* pool;
+    const int *page_table, *positions, *seq_of;
+    void *k_out, *v_out;
+    cudaStream_t stream;
+    int table_stride, page_size, dtype, N, nkv, hd;
+};
+MV_API int mv_kv4_read(const void* record) {
+    const auto& [pool, page_table, positions, seq_of, k_out, v_out, stream, table_stride, page_size, dtype, N, nkv, hd] =
+        *static_cast<const Kv4ReadArgs*>(record);
     if (N <= 0) return 0;
     if (hd % 8 || page_size < 1 || (page_size & (page_size - 1))) return (int)cudaErrorInvalidValue;
     int page_shift = 0;
@@ -633,10 +649,19 @@ attention_kv4_kernel(const T* __restrict__ q, const unsigned char* __restrict__ 
 }
 
 // part_o [N, nh, splits, hd], part_ml [N, nh, splits, 2] float32 and tickets [N, nkv * head_tiles] (zero) are used with splits > 1.
-MV_API int mv_attention_kv4(const void* q, const void* pool, const int* page_table, int table_stride, int page_size,
-                            const int* positions, const int* seq_of, void* o, int dtype, float* part_o, float* part_ml, int* tickets,
-                            int N, int nh, int nkv, int hd, float scale, int window, int splits, int gt, int head_tiles,
-                            cudaStream_t stream) {
+struct AttentionKv4Args {
+    const void *q, *pool;
+    const int *page_table, *positions, *seq_of;
+    void* o;
+    float *part_o, *part_ml;
+    int* tickets;
+    cudaStream_t stream;
+    int table_stride, page_size, dtype, N, nh, nkv, hd, window, splits, gt, head_tiles;
+    float scale;
+};
+MV_API int mv_attention_kv4(const void* record) {
+    const auto& [q, pool, page_table, positions, seq_of, o, part_o, part_ml, tickets, stream, table_stride, page_size, dtype, N, nh, nkv, hd, window, splits,
+                gt, head_tiles, scale] = *static_cast<const AttentionKv4Args*>(record);
     if (N <= 0) return 0;
     if (hd % 8 || hd > KV4_MAX_HEAD_DIM || nkv < 1 || nh % nkv || page_size < 1 || (page_size & (page_size - 1)) || splits < 1 ||
         gt * head_tiles < nh / nkv || N > 65535 || nkv * head_tiles > 65535)

@@ -11,6 +11,7 @@ from __future__ import annotations
 import ctypes
 import functools
 import os
+import struct
 from dataclasses import dataclass
 from typing import Optional, Tuple
 
@@ -30,6 +31,7 @@ class KernelError(RuntimeError):
 
 
 _P, _I, _F, _Q, _UQ = ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.c_longlong, ctypes.c_ulonglong
+_R = ctypes.c_char_p                # a packed record of all arguments: ctypes takes 3.4 us to hand over 30 of them one by one, 1.0 us so
 _SIGNATURES = {
     "core": {
         "mv_embed": [_P, _I, _P, _P, _I, _I, _P],
@@ -48,10 +50,10 @@ _SIGNATURES = {
         "mv_attention_generic": [_P, _P, _Q, _P, _I, _I, _P, _P, _P, _I, _I, _I, _I, _I, _F, _I, _I, _P],
         "mv_attention_decode": [_P, _P, _Q, _P, _I, _I, _P, _P, _P, _I, _P, _P, _P, _I, _I, _I, _I, _F, _I, _I,
                                 _I, _I, _P],
-        "mv_kv4_prepare": [_P, _P, _P, _F, _P, _I, _P, _P, _P, _I, _I, _P, _P, _I, _I, _I, _I, _I, _P],
-        "mv_kv4_read": [_P, _P, _I, _I, _P, _P, _P, _P, _I, _I, _I, _I, _P],
+        "mv_kv4_prepare": [_R],
+        "mv_kv4_read": [_R],
         "mv_kv4_read_pages": [_P, _P, _I, _I, _P, _P, _I, _P, _I, _P, _I, _I, _I, _I, _P],
-        "mv_attention_kv4": [_P, _P, _P, _I, _I, _P, _P, _P, _I, _P, _P, _P, _I, _I, _I, _I, _F, _I, _I, _I, _I, _P],
+        "mv_attention_kv4": [_R],
         "mv_layernorm": [_P, _P, _P, _P, _I, _P, _I, _I, _F, _P],
         "mv_gated_rmsnorm": [_P, _P, _I, _P, _I, _P, _I, _I, _I, _I, _F, _I, _P],
         "mv_rmsnorm_add": [_P, _P, _P, _I, _I, _F, _P],
@@ -136,7 +138,7 @@ _SIGNATURES = {
                                      _P, _P],
         "mv_attention_decode_tc": [_P, _P, _Q, _P, _I, _P, _P, _P, _P, _P, _I, _I, _I, _F, _I, _P, _P],
         "mv_attention_prefill_tc": [_P, _P, _Q, _P, _I, _P, _P, _P, _I, _I, _I, _I, _F, _P, _P],
-        "mv_attention_kv4_decode": [_P, _P, _P, _I, _I, _P, _P, _P, _I, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _F, _I, _I, _I, _I, _I, _I, _I, _I, _P, _P],
+        "mv_attention_kv4_decode": [_R],
         "mv_attention_kv4_prefill": [_P, _P, _P, _I, _I, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _F, _I, _I, _I, _P, _P],
         "mv_latent_attention_decode": [_P, _P, _Q, _P, _I, _I, _P, _P, _P, _P, _I, _I, _I, _I, _F, _I, _I, _P, _P, _P, _P],
         "mv_latent_query": [_P, _I, _I, _P, _P, _P, _I, _I, _I, _I, _I, _F, _P],
@@ -2624,6 +2626,10 @@ def attention_prefill_tc(q: torch.Tensor, pool: torch.Tensor, page_table, cu, st
 
 
 # ---- a cache held in 4 bits --------------------------------------------------------------------------------------
+# the records that the kernels' entries take (Kv4PrepareArgs, Kv4ReadArgs, AttentionKv4Args, AttentionKv4DecodeArgs): pointers, then numbers
+_KV4_PREPARE, _KV4_READ, _KV4_ATTENTION, _KV4_DECODE = (struct.Struct(f).pack for f in ("10P8if0P", "7P6i0P", "10P11if0P", "13P16if0P"))
+
+
 def kv4_page_bytes(page_size: int, hd: int) -> int:
     """Bytes of one kv head in a page held in 4 bits: codes of keys and values, and a step and a zero for every row of each."""
     return page_size * (hd + 8)
@@ -2685,7 +2691,7 @@ def kv4_prepare(qkv: torch.Tensor, wq: Optional[torch.Tensor], wk: Optional[torc
         raise KernelError(f"kv4_prepare: {nh} heads")
     table_shape = _table_shape(page_table, "kv4_prepare")
     dt, dev, f32, i32 = _dt(q_out), qkv.get_device(), torch.float32, torch.int32
-    wq_ptr = wk_ptr = freq_ptr = None
+    wq_ptr = wk_ptr = freq_ptr = 0
     fits = (qkv.dtype is f32 and qkv.shape == (N, (nh + 2 * nkv) * hd) and qkv.is_contiguous() and _is_current(dev)
             and q_out.get_device() == dev and q_out.shape == (N, nh * hd) and q_out.is_contiguous()
             and pool.get_device() == dev and pool.is_contiguous()
@@ -2707,13 +2713,13 @@ def kv4_prepare(qkv: torch.Tensor, wq: Optional[torch.Tensor], wk: Optional[torc
                                 ("page table", page_table, i32, table_shape), ("cache pool", pool, torch.uint8, pool.shape),
                                 ("q out", q_out, q_out.dtype, (N, nh * hd))))
     ptr, out = qkv.data_ptr(), q_out.data_ptr()
-    if (ptr | out | (wq_ptr or 0) | (wk_ptr or 0)) % 16:
+    if (ptr | out | wq_ptr | wk_ptr) % 16:
         raise KernelError("kv4_prepare: qkv, q out and the norm weights must start on 16 bytes")
     if DEBUG_CHECKS:
         _guard("core", "kv4_cache", qkv.device, n_pages=pool.shape[0])
-    _check(_fn("core", "mv_kv4_prepare")(
-        ptr, wq_ptr, wk_ptr, eps, freq_ptr, bool(half_split), positions.data_ptr(), seq_of.data_ptr(),
-        page_table.data_ptr(), table_shape[1], page_size, pool.data_ptr(), out, dt, N, nh, nkv, hd, _stream()), "mv_kv4_prepare")
+    _check(_fn("core", "mv_kv4_prepare")(_KV4_PREPARE(
+        ptr, wq_ptr, wk_ptr, freq_ptr, positions.data_ptr(), seq_of.data_ptr(), page_table.data_ptr(), pool.data_ptr(), out, _stream(),
+        bool(half_split), table_shape[1], page_size, dt, N, nh, nkv, hd, eps)), "mv_kv4_prepare")
     if _profile is not None:
         account(_nbytes(qkv, q_out) + N * nkv * (hd + 8))
     return q_out
@@ -2742,8 +2748,9 @@ def kv4_read(pool: torch.Tensor, page_table, positions, seq_of, k_out: torch.Ten
         raise KernelError("kv4_read: k out and v out must start on 16 bytes")
     if DEBUG_CHECKS:
         _guard("core", "kv4_cache", pool.device, n_pages=pool.shape[0])
-    _check(_fn("core", "mv_kv4_read")(pool.data_ptr(), page_table.data_ptr(), table_shape[1], page_size, positions.data_ptr(), seq_of.data_ptr(),
-                                      k_ptr, v_ptr, dt, N, nkv, hd, _stream()), "mv_kv4_read")
+    _check(_fn("core", "mv_kv4_read")(_KV4_READ(
+        pool.data_ptr(), page_table.data_ptr(), positions.data_ptr(), seq_of.data_ptr(), k_ptr, v_ptr, _stream(), table_shape[1], page_size, dt, N, nkv,
+        hd)), "mv_kv4_read")
     if _profile is not None:
         account(N * nkv * (hd + 8) + _nbytes(k_out, v_out))
     return k_out, v_out
@@ -2913,24 +2920,26 @@ def _attention_kv4_direct(q, pool, page_table, W, page_size, positions, seq_of, 
         flag = _error_flags.get(dev)
         if DEBUG_CHECKS:
             _guard("bf16", "attention_kv4_decode", q.device, n_pages=pool.shape[0])
-        _check(_fn("bf16", "mv_attention_kv4_decode")(
-            q.data_ptr() + row, pool.data_ptr(), page_table.data_ptr(), W, page_size, positions.data_ptr() + 4 * n0, seq_of.data_ptr() + 4 * n0,
-            cu.data_ptr(), n0, starts.data_ptr(), out.data_ptr() + row, part_ml + 8 * parts, part_ml, tickets, N, tiles, nh, nkv, hd, scale, window,
-            nt, head_tiles, heads, tokens, piece, blocks, grid, (_error_flag(q.device) if flag is None else flag).data_ptr(), _stream()), "mv_attention_kv4_decode")
+        _check(_fn("bf16", "mv_attention_kv4_decode")(_KV4_DECODE(
+            q.data_ptr() + row, pool.data_ptr(), page_table.data_ptr(), positions.data_ptr() + 4 * n0, seq_of.data_ptr() + 4 * n0, cu.data_ptr(),
+            starts.data_ptr(), out.data_ptr() + row, part_ml + 8 * parts, part_ml, tickets, (_error_flag(q.device) if flag is None else flag).data_ptr(),
+            _stream(), W, page_size, n0, N, tiles, nh, nkv, hd, window, nt, head_tiles, heads, tokens, piece, blocks, grid, scale)),
+            "mv_attention_kv4_decode")
         return
     gt, head_tiles, auto = attention_kv4_plan(N, nh, nkv, W * page_size)
     splits = auto if splits is None else int(splits)
     if N > 65535 or nkv * head_tiles > 65535:
         raise KernelError(f"attention_kv4: {N} tokens and {nkv} kv heads in one launch; each may be 65535 at most")
-    part_o = part_ml = tickets = None
+    part_o = part_ml = tickets = 0
     if splits > 1:
         part_o = ws.get("attn_part_o", (N * nh * splits * hd,), torch.float32).data_ptr()
         part_ml = ws.get("attn_part_ml", (N * nh * splits * 2,), torch.float32).data_ptr()
         tickets = ws.get_zeroed("attn_tickets", (N * nkv * head_tiles,), torch.int32).data_ptr()
-    _guard("core", "kv4_cache", q.device, n_pages=pool.shape[0])
-    _check(_fn("core", "mv_attention_kv4")(
-        q.data_ptr() + row, pool.data_ptr(), page_table.data_ptr(), W, page_size, positions.data_ptr() + 4 * n0, seq_of.data_ptr() + 4 * n0,
-        out.data_ptr() + row, dt, part_o, part_ml, tickets, N, nh, nkv, hd, scale, window, splits, gt, head_tiles, _stream()), "mv_attention_kv4")
+    if DEBUG_CHECKS:
+        _guard("core", "kv4_cache", q.device, n_pages=pool.shape[0])
+    _check(_fn("core", "mv_attention_kv4")(_KV4_ATTENTION(
+        q.data_ptr() + row, pool.data_ptr(), page_table.data_ptr(), positions.data_ptr() + 4 * n0, seq_of.data_ptr() + 4 * n0, out.data_ptr() + row,
+        part_o, part_ml, tickets, _stream(), W, page_size, dt, N, nh, nkv, hd, window, splits, gt, head_tiles, scale)), "mv_attention_kv4")
 
 
 def attention_kv4_prefill_supported(dtype: torch.dtype, hd: int) -> bool:
