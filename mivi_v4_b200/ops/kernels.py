@@ -2695,8 +2695,8 @@ def kv4_prepare(qkv: torch.Tensor, wq: Optional[torch.Tensor], wk: Optional[torc
     fits = (qkv.dtype is f32 and qkv.shape == (N, (nh + 2 * nkv) * hd) and qkv.is_contiguous() and _is_current(dev)
             and q_out.get_device() == dev and q_out.shape == (N, nh * hd) and q_out.is_contiguous()
             and pool.get_device() == dev and pool.is_contiguous()
-            and positions.get_device() == dev and positions.dtype is i32 and positions.shape == (N,) and positions.is_contiguous()
-            and seq_of.get_device() == dev and seq_of.dtype is i32 and seq_of.shape == (N,) and seq_of.is_contiguous()
+            and positions.get_device() == dev and positions.dtype is i32 and positions.numel() == N and positions.is_contiguous()
+            and seq_of.get_device() == dev and seq_of.dtype is i32 and seq_of.numel() == N and seq_of.is_contiguous()
             and page_table.get_device() == dev and page_table.dtype is i32 and page_table.is_contiguous())
     if fits and wq is not None:
         fits = wq.get_device() == dev and wq.dtype is f32 and wq.shape == (hd,) and wq.is_contiguous()
@@ -2736,8 +2736,8 @@ def kv4_read(pool: torch.Tensor, page_table, positions, seq_of, k_out: torch.Ten
     dt, dev, i32, shape = _dt(k_out), pool.get_device(), torch.int32, (N, nkv, hd)
     if not (pool.is_contiguous() and _is_current(dev)
             and page_table.get_device() == dev and page_table.dtype is i32 and page_table.is_contiguous()
-            and positions.get_device() == dev and positions.dtype is i32 and positions.shape == (N,) and positions.is_contiguous()
-            and seq_of.get_device() == dev and seq_of.dtype is i32 and seq_of.shape == (N,) and seq_of.is_contiguous()
+            and positions.get_device() == dev and positions.dtype is i32 and positions.numel() == N and positions.is_contiguous()
+            and seq_of.get_device() == dev and seq_of.dtype is i32 and seq_of.numel() == N and seq_of.is_contiguous()
             and k_out.get_device() == dev and k_out.shape == shape and k_out.is_contiguous()
             and v_out.get_device() == dev and v_out.shape == shape and v_out.is_contiguous()):
         _misfit("kv4_read", (("cache pool", pool, torch.uint8, pool.shape), ("page table", page_table, i32, table_shape),
@@ -2808,10 +2808,10 @@ def attention_kv4(q: torch.Tensor, pool: torch.Tensor, page_table, positions, se
             and out.get_device() == dev and out.shape == shape and out.is_contiguous()
             and pool.get_device() == dev and pool.is_contiguous()
             and page_table.get_device() == dev and page_table.dtype is i32 and page_table.is_contiguous()
-            and positions.get_device() == dev and positions.dtype is i32 and positions.shape == (N,) and positions.is_contiguous()
-            and seq_of.get_device() == dev and seq_of.dtype is i32 and seq_of.shape == (N,) and seq_of.is_contiguous()
-            and cu.get_device() == dev and cu.dtype is i32 and cu.shape == (B + 1,) and cu.is_contiguous()
-            and starts.get_device() == dev and starts.dtype is i32 and starts.shape == (B,) and starts.is_contiguous()):
+            and positions.get_device() == dev and positions.dtype is i32 and positions.numel() == N and positions.is_contiguous()
+            and seq_of.get_device() == dev and seq_of.dtype is i32 and seq_of.numel() == N and seq_of.is_contiguous()
+            and cu.get_device() == dev and cu.dtype is i32 and cu.numel() == B + 1 and cu.is_contiguous()
+            and starts.get_device() == dev and starts.dtype is i32 and starts.numel() == B and starts.is_contiguous()):
         _misfit("attention_kv4", (("q", q, dtype, shape), ("cache pool", pool, torch.uint8, pool.shape), ("page table", page_table, i32, table_shape),
                                   ("positions", positions, i32, (N,)), ("seq_of", seq_of, i32, (N,)), ("cu", cu, i32, (B + 1,)),
                                   ("starts", starts, i32, (B,)), ("attention out", out, dtype, shape)))
@@ -2881,7 +2881,10 @@ def attention_kv4_decode_plan(N: int, nh: int, nkv: int, hd: int, max_len: int):
     in runs of at most ``max_len``.  A tile's columns are tokens by heads; more columns share a key's way from memory and into
     operands, and cost registers.  The kernel cuts the keys into equal pieces by the lengths that it finds."""
     G = nh // nkv
-    nt_max = 4 if hd <= 128 else 2
+    # (few columns in all: narrow tiles, which more blocks take and whose parts are put together sooner.  16 / 1 heads of 64, one token: 1, 4 and 8
+    # sequences of 8,000 take 10.5, 12.4 and 12.9 us so, 16.2, 17.8 and 18.6 us in tiles of 16 columns; 32 of them 24.6 and 18.8 us.  Between,
+    # 16 tokens of one sequence, 32 / 8 heads: behind 300 5.8, 6.7 and 8.8 us in tiles of 4, 8 and 16, behind 8,000 24.3, 19.0 and 19.4 us.)
+    nt_max = 1 if N * nh <= 256 else 2 if N * nh <= 512 or hd > 128 else 4
     head_tiles = -(-G // (4 * nt_max))
     heads = -(-G // head_tiles)
     tokens = max(1, min(max_len, 4 * nt_max // heads)) if head_tiles == 1 else 1
