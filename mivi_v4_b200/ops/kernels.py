@@ -2802,6 +2802,8 @@ def attention_kv4(q: torch.Tensor, pool: torch.Tensor, page_table, positions, se
         raise KernelError(f"attention_kv4: scale {scale}, expected a positive number")
     if splits is not None and not 1 <= int(splits) <= 1024:
         raise KernelError(f"attention_kv4: {splits} key splits, expected 1..1024")
+    if not -1 < window <= 0x7fffffff:
+        window = 0 if window < 0 else 0x7fffffff
     rows, W = table_shape = _table_shape(page_table, "attention_kv4")
     dt, dev, i32, dtype, shape = _dt(q), q.get_device(), torch.int32, q.dtype, (N, nh * hd)
     if not (q.shape == shape and q.is_contiguous() and _is_current(dev)

@@ -194,3 +194,17 @@ def test_float32_and_small_pages(dtype, nh, nkv, hd, page, window, lens, before)
     q = torch.randn(sum(lens), nh, hd, generator=torch.Generator().manual_seed(8)).to(dtype)
     out = attend_all(q, pool.to(DEV), rows, lengths, lens, nh, nkv, hd, page, window)
     check(out, q, rk, rv, rows, lengths, lens, page, window, dtype, pages=max(lens) > K().KV4_DIRECT_INSTEAD)
+
+
+@pytest.mark.parametrize("nh,nkv,hd,page,window", [(16, 1, 64, 64, 0), (32, 1, 64, 16, 0), (12, 1, 48, 32, 70), (20, 1, 96, 64, 0), (16, 2, 128, 64, 0),
+                                                   (24, 1, 256, 16, 0), (64, 4, 64, 64, 1 << 40), (6, 1, 16, 64, -1)])
+@pytest.mark.parametrize("splits", [None, 3])
+def test_many_single_tokens(nh, nkv, hd, page, window, splits):
+    """Enough columns of queries for wide tiles: many heads of a kv head, in one tile or several."""
+    lengths = [1 + (37 * b) % 400 for b in range(70)]
+    lens = [1] * len(lengths)
+    rows, total = tables(lengths, page, seed=hd)
+    pool, rk, rv = filled(total, nkv, page, hd, seed=nh)
+    q = (2 * torch.randn(len(lengths), nh, hd, generator=torch.Generator().manual_seed(2))).bfloat16()
+    out = attend_all(q, pool.to(DEV), rows, lengths, lens, nh, nkv, hd, page, window, splits=splits)
+    check(out, q, rk, rv, rows, lengths, lens, page, 0 if window > 10 ** 6 else window, torch.bfloat16)
