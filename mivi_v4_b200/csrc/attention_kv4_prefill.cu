@@ -20,7 +20,8 @@
 //                  128-byte swizzle.  A word's eight codes come out as pairs (0, 4), (1, 5), (2, 6), (3, 7) by masking them into the mantissa of
 //                  1024 or 64 and a subtraction; they are left in that order, in which queries are stored too and results are read.
 //   warps 4 - 11   queries to shared memory, then softmax, four warps a half, a row a thread: as in attention_prefill_tc.cu;
-//   warp 12        products, for either half: S = Q K^T (128 x 128 x 64), O += P V (128 x 64 x 128); S(j + 1) runs under the softmax of S(j).
+//   warp 12        products, for either half: S = Q K^T (128 x 128 x 64), O += P V (128 x 64 x 128); S(j + 1) runs under the softmax of S(j);
+//   warp 13        what the block works on next, up to four tiles ahead (warps 14 and 15 only fill the warpgroup that gives its registers away).
 //
 // What bounds it: a key block of a tile takes 3,900 clocks of a multiprocessor, of which the 32,768 exponentials are 2,400 (16 a clock at best;
 // measured 9.4 clocks a warp's instruction with two warps a scheduler), and a row's way from scores to weights is some 3,700 when

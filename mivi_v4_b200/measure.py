@@ -27,7 +27,7 @@ def model_numbers(model, cache_dtype: Optional[str] = None) -> dict:
     head, and the attention operations of a prompt of T tokens."""
     elt = 2 if model.dtype == torch.bfloat16 else 4
     plan = model.cache_plan(cache_dtype)
-    kv_per_token = sum(g.n_layers * g.need.n_kv_heads * (g.need.head_dim + 8 if g.need.bits else (g.need.head_dim + g.need.value_dim) * elt)
+    kv_per_token = sum(g.n_layers * g.need.n_kv_heads * (K.kv4_page_bytes(1, g.need.head_dim) if g.need.bits else (g.need.head_dim + g.need.value_dim) * elt)
                        for g in plan.groups if isinstance(g.need, KVNeed))
     state_per_seq = sum(g.n_layers * torch.empty(0, dtype=g.need.dtype).element_size() * math.prod(g.need.shape)
                         for g in plan.groups if not isinstance(g.need, KVNeed))
