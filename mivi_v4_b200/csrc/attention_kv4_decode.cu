@@ -17,8 +17,10 @@
 //
 // Weights times values: m16n8k16 in half precision, whose 11 bits a weight needs (whole numbers of 15 bits lose those that lie far below the
 // largest).  Codes less 8 are exact in it and cost 1.25 instructions a code: merge two keys' words, mask a nibble of each into the mantissas
-// of 1024 or 64, subtract.  Half's range is small, so the weights p * step are taken relative to the largest step's power of two so far
-// (those whose step is 2^-24 of the largest vanish: so would their values beside the others' in bfloat16).
+// of 1024 or 64, subtract.  Half's range is small, so the weights p * step are taken relative to a power of two: the largest step's so far,
+// while no step is below 2^-KD_SPREAD of it.  Where steps lie further apart, the largest step may be a row's that a column does not see or gives no
+// weight, beside which the rows that it does weigh would vanish; there each column has a unit of its own, which follows the most that one of
+// its rows brings (score and step together).
 //
 // The scores are computed transposed, S^T = K Q^T, keys on a product's 16 rows.  Sums over a row run over elements in any order, so a lane
 // takes the row's bytes as they lie (lane t of four: a quarter of it) and reads its queries to match.  O^T = V^T P^T: a lane takes 8
@@ -49,6 +51,9 @@ namespace {
 // A piece has a tile for every warp at least; up to KD_WHOLE tiles of keys are not cut: a second tile a warp costs less than the meeting of two
 // blocks (300 rows of one sequence: 5.0 us whole, 6.6 us in two; 1,000 rows behind a window: 10.8 us in pieces of 8, 9.6 us in pieces of 4).
 constexpr int KD_WARPS = 4, KD_KEYS = 64, KD_WHOLE = 8;
+// A weight p * step is at most 2^15 in a column's unit (p up to 2^8, the step below 2 of them times 2^6); steps that lie further apart than
+// 2^KD_SPREAD are not weighed in one unit.
+constexpr int KD_ROOM = 6, KD_SPREAD = 8, KD_UNIT_MIN = -120;
 
 __device__ __forceinline__ void bulk_load(unsigned dst, const void* src, unsigned bytes, unsigned bar) {
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
@@ -311,10 +316,15 @@ attention_kv4_decode_kernel(const __nv_bfloat16* __restrict__ q, const unsigned 
 
     float oacc[NT][MT][4];
     float m[NT], l[NT], pz[NT];                                  // maxima (log2 units, alike in all rows' lanes), this lane's sums
-    int ev = -126;                                               // the weights' power of two, and its inverse
-    float ev_down = pow2f(126);
+    // the power of two of the largest step so far, times 2^-KD_ROOM: the unit of all columns' weights, until steps lie far apart (wide); of each
+    // column's unit the inverse; this lane's least step so far
+    int ev = KD_UNIT_MIN;
+    float down[NT];
+    unsigned low = 0xffffffffu;
+    bool wide = false;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
+        down[nt] = pow2f(-KD_UNIT_MIN);
         m[nt] = -INFINITY;
         l[nt] = pz[nt] = 0.f;
 #pragma unroll
@@ -339,7 +349,7 @@ attention_kv4_decode_kernel(const __nv_bfloat16* __restrict__ q, const unsigned 
 
         // ---- scores, in units of the columns' own: 64 keys x 4 NT columns; s[nt][r]: key 8 r + key_of
         float s[NT][8], sv[8], zv[8];
-        unsigned smax = 0u;
+        unsigned smax = 0u, smin = 0xffffffffu;
 #pragma unroll
         for (int b = 0; b < 4; ++b) {
             int dot[NT][4];
@@ -378,19 +388,25 @@ attention_kv4_decode_kernel(const __nv_bfloat16* __restrict__ q, const unsigned 
                 const Kv4Params p = kv4_params(pt[16 * b + 8 * j + key_of]);
                 sv[2 * b + j] = p.vs;
                 zv[2 * b + j] = fmaf(8.f, p.vs, p.vz);
-                smax = max(smax, __float_as_uint(p.vs));
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
                     s[nt][2 * b + j] = fmaf((float)(dot[nt][2 * j] * 256 + dot[nt][2 * j + 1]), p.ks * unit[nt], p.kz * qsum[nt]);
             }
         }
+#pragma unroll
+        for (int r = 0; r < 8; r += 2) {
+            smax = __vimax3_u32(smax, __float_as_uint(sv[r]), __float_as_uint(sv[r + 1]));
+            smin = __vimin3_u32(smin, __float_as_uint(sv[r]), __float_as_uint(sv[r + 1]));
+        }
         // ---- at the edges: keys that some column, or none, sees
         if (key0 + KD_KEYS - 1 > pos0 || (window > 0 && key0 <= pos_last - window)) {
             smax = 0u;
+            smin = 0xffffffffu;
 #pragma unroll
             for (int r = 0; r < 8; ++r) {
                 const int at = key0 + 8 * r + key_of;
                 if (at > pos_last || at < lo_key) sv[r] = zv[r] = 0.f;
+                else smin = min(smin, __float_as_uint(sv[r]));
                 smax = max(smax, __float_as_uint(sv[r]));
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
@@ -415,20 +431,26 @@ attention_kv4_decode_kernel(const __nv_bfloat16* __restrict__ q, const unsigned 
             }
             smax = __reduce_max_sync(0xffffffffu, smax);
         }
-        const int ev_new = max(ev, (int)(smax >> 23) - 127);
-        if (ev_new != ev) {                                      // (as a rule only in the first tiles)
+        // (where no step is 2^KD_SPREAD times another, a column's best key has a weight within that of the largest there can be, whichever rows
+        // the column sees: its others keep 11 bits down to 2^-12 of it, and lose what is below 2^-23 of it)
+        low = min(low, smin);
+        const int ev_new = max(ev, (int)(smax >> 23) - 127 - KD_ROOM);
+        // (and weights beyond 2^118, which times 2^8 could pass the largest float, are taken relative to the maximum at once)
+        if (__any_sync(0xffffffffu, low < (unsigned)(ev_new + KD_ROOM - KD_SPREAD + 127) << 23) || ev_new + KD_ROOM > 117) wide = true;
+        if (ev_new != ev && !wide) {                             // (as a rule only in the first tiles)
             const float f = ev_new - ev > 126 ? 0.f : pow2f(ev - ev_new);
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
+            for (int nt = 0; nt < NT; ++nt) {
+                down[nt] = pow2f(-ev_new);
 #pragma unroll
                 for (int k = 0; k < MT; ++k)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) oacc[nt][k][e] *= f;
-            ev = ev_new;
-            ev_down = pow2f(-ev);
+            }
         }
+        ev = ev_new;
         // ---- maxima: a column's reference moves when a score passes it by 2^8, for all columns of the warp together
-        bool moves = false;
+        bool moves = wide;
         float mx[NT];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
@@ -445,6 +467,22 @@ attention_kv4_decode_kernel(const __nv_bfloat16* __restrict__ q, const unsigned 
                 for (int d = 4; d < 32; d <<= 1) mx[nt] = fmaxf(mx[nt], __shfl_xor_sync(0xffffffffu, mx[nt], d));
                 mx[nt] = fmaxf(mx[nt], m[nt]);
                 const float corr = m[nt] == -INFINITY ? 0.f : ex2(m[nt] - mx[nt]);
+                float of = corr;
+                if (wide) {
+                    // the column's own unit: the most that a row which it sees can bring, its weight times its step, is 2^14 of it or less; it never
+                    // falls, relative to 1
+                    float my = -INFINITY;
+#pragma unroll
+                    for (int r = 0; r < 8; ++r)
+                        if (sv[r] > 0.f) my = fmaxf(my, __fmul_rn(s[nt][r], lsc[nt]) - mx[nt] + (float)((int)(__float_as_uint(sv[r]) >> 23) - 126));
+#pragma unroll
+                    for (int d = 4; d < 32; d <<= 1) my = fmaxf(my, __shfl_xor_sync(0xffffffffu, my, d));
+                    const int unit = 127 - (int)(__float_as_uint(down[nt]) >> 23);
+                    const int to = max((int)ceilf(fmaxf(my, -400.f)) - 14, (int)ceilf(fmaxf((float)unit + (m[nt] - mx[nt]), -400.f)));
+                    const int unit_new = min(max(to, KD_UNIT_MIN), 121);
+                    of = m[nt] == -INFINITY ? 0.f : ex2(m[nt] - mx[nt] + (float)(unit - unit_new));
+                    down[nt] = pow2f(-unit_new);
+                }
                 m[nt] = mx[nt];
                 l[nt] *= corr;
                 pz[nt] *= corr;
@@ -452,7 +490,7 @@ attention_kv4_decode_kernel(const __nv_bfloat16* __restrict__ q, const unsigned 
 #pragma unroll
                 for (int k = 0; k < MT; ++k)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) oacc[nt][k][e] *= corr;
+                    for (int e = 0; e < 4; ++e) oacc[nt][k][e] *= of;
             }
         }
         // ---- weights and the values' product, 32 keys at a time
@@ -471,7 +509,7 @@ attention_kv4_decode_kernel(const __nv_bfloat16* __restrict__ q, const unsigned 
                         const float p = ex2(fmaf(s[nt][r], lsc[nt], ref));  // (ex2(-infinity) is 0: a key that is not seen)
                         l[nt] += p;
                         pz[nt] = fmaf(p, zv[r], pz[nt]);
-                        w[k] = p * (sv[r] * ev_down);
+                        w[k] = p * sv[r] * down[nt];
                     }
                     const unsigned x = transpose8x8(half_pair(w[0], w[1]));
                     pe[nt][j] = g & 1 ? 0u : x;
@@ -510,9 +548,9 @@ attention_kv4_decode_kernel(const __nv_bfloat16* __restrict__ q, const unsigned 
     float* xo = reinterpret_cast<float*>(smem);                  // [warp][column][HDP], then maxima and sums [warp][column]
     float* xm = xo + KD_WARPS * COLS * HDP;
     float* xl = xm + KD_WARPS * COLS;
-    const float up = pow2f(ev);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
+        const float up = 1.0f / down[nt];
 #pragma unroll
         for (int d = 4; d < 32; d <<= 1) {
             l[nt] += __shfl_xor_sync(0xffffffffu, l[nt], d);
