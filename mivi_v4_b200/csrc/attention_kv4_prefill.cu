@@ -6,7 +6,9 @@
 // and the result by 0.004 where its own rounding is 0.0017; with 11 bits it is 0.0017.  Half's range is small, so powers of two are taken
 // out: of a query row its largest element's, of every 32 keys, and of every 32 values, their largest element's (from the rows' numbers:
 // a row's ends are zero and zero + 15 steps).  Those of the keys go into the factor of the exponential, those of the values into the
-// exponent of the weights, relative to the largest so far.
+// exponent of the weights, relative to a power of two of the query's own: the most that a row it sees brings so far, score and size together
+// (a row that it does not see, or gives no weight, would push the others' weights below half's range).  Where the rows of 32 lie further apart
+// than 2^KQ_SPREAD, each has powers of two of its own: such a key block is uneven, and the softmax warps take its scores one by one.
 //
 // A tile is 256 query rows of one kv head, as two halves of 128 rows: rows are tokens by the heads that share the kv head, so its keys are
 // turned into operands once for all of them, a run of a few dozen tokens fills a half, and little is spent on keys that only some rows see.
@@ -46,11 +48,16 @@ constexpr int BQ = 128, TILES = 2, ROWS = BQ * TILES, BKV = 128, HD = 64;
 constexpr int Q_BYTES = BQ * HD * 2, KV_BYTES = BKV * HD * 2, P_BYTES = BQ * BKV * 2;
 constexpr int STAGES = 3, EXPS = 8, KQ_MOST = 1024;              // most sequences, and most tiles, of a launch
 constexpr int KQ_EXTRA = 3;                                      // key blocks that a tile's beginning and end count for
+constexpr int UNEVEN = 0x7f800000;
+constexpr int KQ_SPREAD = 8;                                     // rows of 32 whose sizes are within this many powers of two share theirs
 constexpr int KQ_BARS = TILES * Q_BYTES + 2 * STAGES * KV_BYTES + TILES * P_BYTES, KQ_EXPS = KQ_BARS + 272, KQ_SEGS = KQ_EXPS + EXPS * 32, KQ_TABLES = KQ_SEGS + 4 * 96,
-              KQ_SMEM = KQ_TABLES + (3 * KQ_MOST + 4) * 4 + 1024;
+              KQ_OWN = KQ_TABLES + (3 * KQ_MOST + 4) * 4, KQ_SMEM = KQ_OWN + EXPS * BKV * 4 + 1024;
 static_assert(KQ_SMEM <= 227 * 1024 - 512, "shared memory");
 constexpr unsigned S_COL0 = 0, O_COL0 = 256;                     // of half t: S 128 t on, O 64 t on
-constexpr float RESCALE_ABOVE = 8.0f;
+static_assert(KQ_OWN % 16 == 0, "read 16 bytes at a time");
+// A row's weights are at most 2^(RESCALE_ABOVE + WEIGHT_ROOM) in its unit, which half precision holds; beside the largest so far they keep their
+// 11 bits down to 2^-21 of it, and what is below 2^-32 of it is lost.
+constexpr float RESCALE_ABOVE = 8.0f, WEIGHT_ROOM = 7.0f;
 
 enum { B_Q = 0, B_KFULL = B_Q + TILES, B_KEMPTY = B_KFULL + STAGES, B_VFULL = B_KEMPTY + STAGES, B_VEMPTY = B_VFULL + STAGES,
        B_SFULL = B_VEMPTY + STAGES, B_PFULL = B_SFULL + TILES, B_PVDONE = B_PFULL + TILES, B_SFREE = B_PVDONE + TILES, B_SEGFULL = B_SFREE + TILES, B_SEGEMPTY = B_SEGFULL + 4,
@@ -133,7 +140,8 @@ attention_kv4_prefill_kernel(const __nv_bfloat16* __restrict__ q, const unsigned
     unsigned long long* bars = (unsigned long long*)(smem + KQ_BARS);
     unsigned* tmem_holder = (unsigned*)(bars + B_COUNT);
     Segment* segs = reinterpret_cast<Segment*>(smem + KQ_SEGS);  // the segments to come, a ring of four (worked out by a warp of its own)
-    int2* exps = reinterpret_cast<int2*>(smem + KQ_EXPS);        // [key block][32 keys]: powers of two of the keys, of the values
+    int2* exps = reinterpret_cast<int2*>(smem + KQ_EXPS);        // [key block][32 keys]: powers of two of the keys, of the values (a float, or UNEVEN)
+    int* own = reinterpret_cast<int*>(smem + KQ_OWN);            // [key block][key]: the same of each key where they are uneven, 16 bits each
     int* seq_first = reinterpret_cast<int*>(smem + KQ_TABLES);   // [sequence + 1]: its first tile
     int* before = seq_first + KQ_MOST + 1;                       // [tile + 1]: key blocks of the tiles before it
     int* seq_of_tile = before + KQ_MOST + 1;
@@ -355,14 +363,22 @@ attention_kv4_prefill_kernel(const __nv_bfloat16* __restrict__ q, const unsigned
                 const unsigned ph = (unsigned)(it / STAGES) & 1u;
                 Kv4Params p = kv4_params(np);
                 kv4_poison(p);
+                const bool there = from != nullptr;
                 if (j + 1 < g.n) {
                     place_of(g.kb + j + 1);
                     fetch_numbers();
                 }
                 // powers of two of the warp's keys and values (a row that is not finite has no say)
                 const float big_k = fmaxf(fabsf(p.kz), fabsf(fmaf(15.f, p.ks, p.kz))), big_v = fmaxf(fabsf(p.vz), fabsf(fmaf(15.f, p.vs, p.vz)));
-                const int ek = exponent(__reduce_max_sync(0xffffffffu, big_k < INFINITY ? __float_as_uint(big_k) : 0u));
-                const int ev = exponent(__reduce_max_sync(0xffffffffu, __float_as_uint(big_v)));
+                const unsigned bits_k = big_k < INFINITY ? __float_as_uint(big_k) : 0u, bits_v = __float_as_uint(big_v);
+                const unsigned top_k = __reduce_max_sync(0xffffffffu, bits_k), top_v = __reduce_max_sync(0xffffffffu, bits_v);
+                int ek = exponent(top_k), ev = exponent(top_v);
+                // (a key of zeros scores 0 in any unit; a value of zeros may have the weight that the others' are to be measured by)
+                const bool uneven = __any_sync(0xffffffffu, there && ((bits_k != 0u && bits_k + (KQ_SPREAD << 23) < top_k) || bits_v + (KQ_SPREAD << 23) < top_v));
+                if (uneven) {
+                    ek = exponent(bits_k);
+                    ev = exponent(bits_v);
+                }
                 auto put = [&](unsigned char* stage, const uint4 (&w)[2], float step, float zero, float down) {
                     const unsigned st = twice(step * down), z = twice(zero * down);
                     unsigned char* to = stage + key_of * 128;
@@ -377,7 +393,8 @@ attention_kv4_prefill_kernel(const __nv_bfloat16* __restrict__ q, const unsigned
                     if (lane == 0) mbar_arrive(bar(b + s));
                 };
                 if (!(ok = mbar_wait_warp(bar(B_KEMPTY + s), ph ^ 1u, err, 161))) break;
-                if (lane == 0) exps[(it % EXPS) * 4 + warp] = make_int2(ek, ev);
+                if (lane == 0) exps[(it % EXPS) * 4 + warp] = make_int2(ek, uneven ? UNEVEN : __float_as_int((float)ev));
+                if (uneven) own[(it % EXPS) * BKV + key_of] = (ek & 0xffff) | (ev << 16);
                 put(k_ptr + s * KV_BYTES, kc, p.ks, p.kz, pow2f(-ek));
                 if (j + 1 < g.n) fetch(kc, 0);
                 hand_over(B_KFULL);
@@ -537,59 +554,44 @@ attention_kv4_prefill_kernel(const __nv_bfloat16* __restrict__ q, const unsigned
                 if (lane == 0) mbar_arrive(bar(B_Q + t));
             }
             float m = -INFINITY, l = fine ? 0.f : NAN;           // m: the row's reference, log2 units
-            int ev = -126;                                       // the accumulator's power of two
-            for (int j = 0; j < my_nb && ok; ++j) {
-                ok = mbar_wait_warp(bar(B_SFULL + t), (unsigned)(done + j) & 1u, err, 169);
-                if (!ok) break;
-                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                unsigned s[4][32];
-                tmem_ld32(s_addr, s[0]);
-                tmem_ld32(s_addr + 32, s[1]);
-                tmem_ld32(s_addr + 64, s[2]);
-                tmem_ld32(s_addr + 96, s[3]);
-                const int2* e = exps + ((it + j) % EXPS) * 4;
-                float f[4];                                      // 32 keys' factor to log2 units
-                int ev_new = ev, d4[4];
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    const int2 x = e[c];
-                    f[c] = scale_log2 * pow2f(max(-126, min(120, ex + x.x)));
-                    d4[c] = x.y;
-                    ev_new = max(ev_new, x.y);
-                }
-                asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+            float rel = 0.f;                                     // the accumulator's unit is 2^(rel - WEIGHT_ROOM) of what weights relative to 2^m come to
+            int j = 0;
+            bool uneven = false;                                 // (the same for all threads)
+            auto hand_over = [&]() {
+                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar(B_PFULL + t));
+            };
+            auto free_scores = [&]() {
                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                 __syncwarp();
                 if (lane == 0) mbar_arrive(bar(B_SFREE + t));
-                const int key0 = (sg->kb + j) * BKV;
-                // warp-uniform: some row of the half does not see the whole block
-                if (key0 + BKV - 1 > sg->first[t] || (window > 0 && key0 <= sg->past[t] - window)) {
-                    const int past = pos - key0 + 1, from = window > 0 ? past - window : 0;
-#pragma unroll
-                    for (int c = 0; c < 4; ++c)
-#pragma unroll
-                        for (int i = 0; i < 32; ++i)
-                            if (32 * c + i >= past || 32 * c + i < from) s[c][i] = 0xff800000u;
-                }
-                float mx = -INFINITY;
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    float a[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-                    for (int i = 0; i < 32; i += 2) a[(i >> 1) & 3] = max3(a[(i >> 1) & 3], __uint_as_float(s[c][i]), __uint_as_float(s[c][i + 1]));
-                    mx = fmaxf(mx, max3(a[0], a[1], fmaxf(a[2], a[3])) * f[c]);
-                }
-                float corr = 1.0f;                               // of the row's sum
+            };
+            // the row's reference follows its largest score, by 2^RESCALE_ABOVE at least
+            auto follow = [&](float mx) {
                 if (mx > m + RESCALE_ABOVE) {
-                    corr = m == -INFINITY ? 0.f : ex2(m - mx);
+                    l *= m == -INFINITY ? 0.f : ex2(m - mx);
                     m = mx;
                 }
-                const float o_corr = ev_new == ev ? corr : (ev - ev_new < -120 ? 0.f : corr * pow2f(ev - ev_new));
-                ev = ev_new;
+                return m == -INFINITY ? 0.f : m;
+            };
+            // the accumulator's unit follows the most that a row brings (relative to 2^m: its weight times its values' power of two); its factor
+            auto measure = [&](float most, float m_old) {
+                float o_corr = 1.0f;
+                if (m != -INFINITY) {                            // (until then all of its weights are 0, and so is its accumulator)
+                    rel += m_old - m;                            // (from -infinity: it has no unit yet)
+                    if (most > rel + RESCALE_ABOVE) {
+                        o_corr = ex2(rel - most);
+                        rel = most;
+                    }
+                }
+                return o_corr;
+            };
+            auto make_room = [&](float o_corr) {
                 // P (shared memory) and O (tensor memory) are the key block before's until its product is done
                 if (j > 0) {
-                    ok = mbar_wait_warp(bar(B_PVDONE + t), (unsigned)(done + j - 1) & 1u, err, 170);
-                    if (!ok) break;
+                    if (!mbar_wait_warp(bar(B_PVDONE + t), (unsigned)(done + j - 1) & 1u, err, 170)) return false;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 }
                 if (j > 0 && __any_sync(0xffffffffu, o_corr != 1.0f)) {
@@ -604,58 +606,157 @@ attention_kv4_prefill_kernel(const __nv_bfloat16* __restrict__ q, const unsigned
                     }
                     asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                 }
-                const float ref = m == -INFINITY ? 0.f : m;
-                l *= corr;
-                // weights relative to the accumulator's power of two, eight at a time (b); their sums relative to 1
-                auto raise = [&](int b) {
-                    const int c = b >> 2;
-                    const float from = (float)max(-60, d4[c] - ev) - ref;
+                return true;
+            };
+            while (ok && j < my_nb) {
+                uneven = false;
+                for (; j < my_nb; ++j) {
+                    ok = mbar_wait_warp(bar(B_SFULL + t), (unsigned)(done + j) & 1u, err, 169);
+                    if (!ok) break;
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    unsigned s[4][32];
+                    tmem_ld32(s_addr, s[0]);
+                    tmem_ld32(s_addr + 32, s[1]);
+                    tmem_ld32(s_addr + 64, s[2]);
+                    tmem_ld32(s_addr + 96, s[3]);
+                    const int2* e = exps + ((it + j) % EXPS) * 4;
+                    float f[4], ev[4];                           // 32 keys' factor to log2 units, their values' power of two
 #pragma unroll
-                    for (int i = 8 * (b & 3); i < 8 * (b & 3) + 8; i += 2) {
-                        const float2 x = fma2(make_float2(__uint_as_float(s[c][i]), __uint_as_float(s[c][i + 1])), make_float2(f[c], f[c]), make_float2(from, from));
-                        s[c][i] = __float_as_uint(ex2(x.x));
-                        s[c][i + 1] = __float_as_uint(ex2(x.y));
+                    for (int c = 0; c < 4; ++c) {
+                        const int2 x = e[c];
+                        f[c] = scale_log2 * pow2f(max(-126, min(120, ex + x.x)));
+                        ev[c] = __int_as_float(x.y);
+                        uneven = uneven || x.y == UNEVEN;
                     }
-                };
-                float2 sum = make_float2(0.f, 0.f);
-                auto put = [&](int b) {
-                    const int c = b >> 2, q4 = b & 3;
-                    unsigned w[4];
+                    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                    if (uneven) break;
+                    free_scores();
+                    const int key0 = (sg->kb + j) * BKV;
+                    // warp-uniform: some row of the half does not see the whole block
+                    if (key0 + BKV - 1 > sg->first[t] || (window > 0 && key0 <= sg->past[t] - window)) {
+                        const int past = pos - key0 + 1, from = window > 0 ? past - window : 0;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float2 p = make_float2(__uint_as_float(s[c][8 * q4 + 2 * i]), __uint_as_float(s[c][8 * q4 + 2 * i + 1]));
-                        sum = i + q4 ? add2(sum, p) : p;
-                        const __half2 v = __floats2half2_rn(p.x, p.y);
-                        w[i] = *reinterpret_cast<const unsigned*>(&v);
+                        for (int c = 0; c < 4; ++c)
+#pragma unroll
+                            for (int i = 0; i < 32; ++i)
+                                if (32 * c + i >= past || 32 * c + i < from) s[c][i] = 0xff800000u;
                     }
-                    *reinterpret_cast<uint4*>(p_row + (c >> 1) * (BQ * 128) + (((4 * (c & 1) + q4) ^ (r & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
-                    if (q4 == 3) l = fmaf(sum.x + sum.y, pow2f(-max(-60, d4[c] - ev)), l);
-                };
-                // the two warps of a scheduler take turns (a matter of speed only: nothing waits for good)
-                if (t == 0) raising[0][quarter] = 1;
-                for (int k = 0; k < 64 && raising[t ^ 1][quarter]; ++k) ;
-                if (t == 1) raising[1][quarter] = 1;
-                __syncwarp();
-                constexpr int AHEAD = 3;                          // (the unit's latency: 207 us with 1, 204 with 3)
+                    float mx = -INFINITY, top[4];                // top: of 32 keys
 #pragma unroll
-                for (int b = 0; b < AHEAD; ++b) raise(b);
+                    for (int c = 0; c < 4; ++c) {
+                        float a[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                for (int b = 0; b < 16; ++b) {
-                    if (b + AHEAD < 16) raise(b + AHEAD);
-                    if (b + AHEAD == 12) raising[t][quarter] = 0;  // (its last ones are under way when the other comes)
-                    put(b);
+                        for (int i = 0; i < 32; i += 2) a[(i >> 1) & 3] = max3(a[(i >> 1) & 3], __uint_as_float(s[c][i]), __uint_as_float(s[c][i + 1]));
+                        top[c] = max3(a[0], a[1], fmaxf(a[2], a[3])) * f[c];
+                        mx = fmaxf(mx, top[c]);
+                    }
+                    const float m_old = m, ref = follow(mx);
+                    float most = -INFINITY;
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) most = fmaxf(most, top[c] - ref + ev[c]);
+                    const float o_corr = measure(most, m_old);
+                    // exponent of 32 keys' weights less that of their scores, and what brings their sum back to 2^m
+                    float lift[4], back[4];
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        lift[c] = fmaxf(ev[c] - rel + WEIGHT_ROOM, -60.f);
+                        back[c] = ex2(-lift[c]);
+                    }
+                    if (!(ok = make_room(o_corr))) break;
+                    // weights relative to the accumulator's unit, eight at a time (b); their sums relative to 2^m
+                    auto raise = [&](int b) {
+                        const int c = b >> 2;
+                        const float from = lift[c] - ref;
+#pragma unroll
+                        for (int i = 8 * (b & 3); i < 8 * (b & 3) + 8; i += 2) {
+                            const float2 x = fma2(make_float2(__uint_as_float(s[c][i]), __uint_as_float(s[c][i + 1])), make_float2(f[c], f[c]), make_float2(from, from));
+                            s[c][i] = __float_as_uint(ex2(x.x));
+                            s[c][i + 1] = __float_as_uint(ex2(x.y));
+                        }
+                    };
+                    float2 sum = make_float2(0.f, 0.f);
+                    auto put = [&](int b) {
+                        const int c = b >> 2, q4 = b & 3;
+                        unsigned w[4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const float2 p = make_float2(__uint_as_float(s[c][8 * q4 + 2 * i]), __uint_as_float(s[c][8 * q4 + 2 * i + 1]));
+                            sum = i + q4 ? add2(sum, p) : p;
+                            const __half2 v = __floats2half2_rn(p.x, p.y);
+                            w[i] = *reinterpret_cast<const unsigned*>(&v);
+                        }
+                        *reinterpret_cast<uint4*>(p_row + (c >> 1) * (BQ * 128) + (((4 * (c & 1) + q4) ^ (r & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+                        if (q4 == 3) l = fmaf(sum.x + sum.y, back[c], l);
+                    };
+                    // the two warps of a scheduler take turns (a matter of speed only: nothing waits for good)
+                    if (t == 0) raising[0][quarter] = 1;
+                    for (int k = 0; k < 64 && raising[t ^ 1][quarter]; ++k) ;
+                    if (t == 1) raising[1][quarter] = 1;
+                    __syncwarp();
+                    constexpr int AHEAD = 3;                          // (the unit's latency: 207 us with 1, 204 with 3)
+#pragma unroll
+                    for (int b = 0; b < AHEAD; ++b) raise(b);
+#pragma unroll
+                    for (int b = 0; b < 16; ++b) {
+                        if (b + AHEAD < 16) raise(b + AHEAD);
+                        if (b + AHEAD == 12) raising[t][quarter] = 0;  // (its last ones are under way when the other comes)
+                        put(b);
+                    }
+                    hand_over();
                 }
-                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                __syncwarp();
-                if (lane == 0) mbar_arrive(bar(B_PFULL + t));
+                if (!ok || !uneven) break;
+                // Every key has powers of two of its own: its score is taken by itself, and its weight and its values' size are added up apart.  (A
+                // path of its own, outside of the loop, which reads the scores from tensor memory again.  400 and 700 tokens behind 6,000 and 12,000, which
+                // never come here, take 163 us so, 214 us where the scores are held in registers through it, and 159 us without it.)
+                const int past = pos - (sg->kb + j) * BKV + 1, from = window > 0 ? past - window : 0;
+                auto each = [&](auto use) {                      // use(32 keys, i, score in log2 units, its values' power of two)
+#pragma unroll 1
+                    for (int c = 0; c < 4; ++c) {
+                        unsigned x[32];
+                        tmem_ld32(s_addr + 32u * (unsigned)c, x);
+                        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                        const int2 shared = exps[((it + j) % EXPS) * 4 + c];
+                        const int* own_of = own + ((it + j) % EXPS) * BKV + 32 * c;
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) {
+                            const int k = own_of[i], ek = shared.y == UNEVEN ? (int)(short)k : shared.x;
+                            const float v = shared.y == UNEVEN ? (float)(k >> 16) : __int_as_float(shared.y);
+                            const bool seen = 32 * c + i < past && 32 * c + i >= from;
+                            use(c, i, seen ? __fmul_rn(__uint_as_float(x[i]), scale_log2 * pow2f(max(-126, min(120, ex + ek)))) : -INFINITY, v);
+                        }
+                    }
+                };
+                float mx = -INFINITY, most = -INFINITY, sum = 0.f;
+                each([&](int, int, float x, float) { mx = fmaxf(mx, x); });
+                const float m_old = m, ref = follow(mx);
+                each([&](int, int, float x, float v) {
+                    sum += ex2(x - ref);
+                    most = fmaxf(most, x - ref + v);
+                });
+                l += sum;
+                if (!(ok = make_room(measure(most, m_old)))) break;
+                unsigned w[4];
+                float first = 0.f;
+                each([&](int c, int i, float x, float v) {
+                    const float p = ex2(x - ref + (v - rel + WEIGHT_ROOM));
+                    if (i & 1) {
+                        const __half2 h = __floats2half2_rn(first, p);
+                        w[(i >> 1) & 3] = *reinterpret_cast<const unsigned*>(&h);
+                    }
+                    first = p;
+                    if ((i & 7) == 7) *reinterpret_cast<uint4*>(p_row + (c >> 1) * (BQ * 128) + (((4 * (c & 1) + (i >> 3)) ^ (r & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+                });
+                free_scores();
+                hand_over();
+                ++j;
             }
             if (ok && my_nb > 0) ok = mbar_wait_warp(bar(B_PVDONE + t), (unsigned)(done + my_nb - 1) & 1u, err, 171);
             if (ok && my_nb > 0) asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             if (!ok) break;
             // ---- the rows out, by the queries' place in shared memory (a warp's own rows: whole lines leave), or a part of them
             const bool read = ok && my_nb > 0;
-            const float up = pow2f(ev) * (parts == 1 ? 1.0f / l : 1.0f);
+            // (in two factors: the unit may lie beyond the floats where the result does not.  A part is divided by its sum, too: it may pass them before.)
+            const float up0 = ex2(0.5f * (rel - WEIGHT_ROOM)), up1 = l == 0.f ? 0.f : up0 / l;
             // a block has two parts at most: of a tile that it begins, and of one that another block began
             const int slot = 2 * blockIdx.x + (sg->c1 == (int)blockIdx.x ? 1 : 0);
             float4* mine = reinterpret_cast<float4*>(part_o) + (size_t)slot * (ROWS * HD / 4) + t * BQ + r;
@@ -674,7 +775,7 @@ attention_kv4_prefill_kernel(const __nv_bfloat16* __restrict__ q, const unsigned
                     for (int d = 0; d < 32; d += 8) {            // stored as 0, 4, 1, 5, 2, 6, 3, 7
                         float x[8];
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) x[i] = __uint_as_float(v[d + i]) * up;
+                        for (int i = 0; i < 8; ++i) x[i] = __uint_as_float(v[d + i]) * up0 * up1;
                         if (parts == 1) {
                             const uint4 w = make_uint4(bits(__floats2bfloat162_rn(x[0], x[2])), bits(__floats2bfloat162_rn(x[4], x[6])),
                                                        bits(__floats2bfloat162_rn(x[1], x[3])), bits(__floats2bfloat162_rn(x[5], x[7])));
@@ -717,7 +818,7 @@ attention_kv4_prefill_kernel(const __nv_bfloat16* __restrict__ q, const unsigned
                 ++merges;
                 const bool last = is_last;
                 if (last && t * BQ < sg->nq) {
-                    // A part: reference (log2 units), sum, weighted values.  Where nothing was seen the sum is 0 and the part counts nothing;
+                    // A part: reference (log2 units), sum, mean of the values.  Where nothing was seen the sum is 0 and the part counts nothing;
                     // where all that was seen is not a number the sum is not one, and stays so.
                     auto weight = [](float mx, float sum, float M) { return mx == -INFINITY ? (sum == 0.f ? 0.f : NAN) : ex2(mx - M); };
                     const int row = t * BQ + r, c1 = sg->c1;
@@ -730,8 +831,8 @@ attention_kv4_prefill_kernel(const __nv_bfloat16* __restrict__ q, const unsigned
                         for (int p = 0; p < parts; ++p) M = fmaxf(M, __ldcg(part_ml + ((size_t)slot_of(p) * ROWS + row) * 2));
                         for (int p = 0; p < parts; ++p) {
                             const float2 ml = __ldcg(reinterpret_cast<const float2*>(part_ml + ((size_t)slot_of(p) * ROWS + row) * 2));
-                            const float w = weight(ml.x, ml.y, M);
-                            L = fmaf(ml.y, w, L);
+                            const float w = ml.y * weight(ml.x, ml.y, M);
+                            L += w;
                             const float4* from = reinterpret_cast<const float4*>(part_o) + (size_t)slot_of(p) * (ROWS * HD / 4) + row;
 #pragma unroll
                             for (int c = 0; c < HD / 4; ++c) {

@@ -105,6 +105,12 @@ SHAPES = {
     "short runs": (torch.bfloat16, 8, 2, 64, 64, 0, [4, 16, 1], [100, 3, 260], None),
     "short runs, window": (torch.bfloat16, 4, 4, 64, 16, 10, [14, 9], [200, 3], None),
     "short runs, many": (torch.bfloat16, 8, 1, 64, 64, 0, [13] * 24, [5 * b for b in range(24)], None),
+    "many tokens": (torch.bfloat16, 8, 2, 64, 64, 0, [200, 33, 7], [0, 300, 20], "planned"),
+    "many tokens, whole": (torch.bfloat16, 4, 2, 64, 16, 0, [270], [130], "whole"),
+    "many tokens, shared": (torch.bfloat16, 4, 2, 64, 64, 0, [270, 40], [130, 500], "shared"),
+    "many tokens, few blocks": (torch.bfloat16, 6, 2, 64, 64, 30, [270, 40], [130, 500], "few blocks"),
+    "many tokens, window": (torch.bfloat16, 3, 1, 64, 1, 40, [300], [100], "planned"),
+    "many tokens, small head": (torch.bfloat16, 6, 2, 48, 64, 0, [100, 140], [200, 0], "shared"),
     "many tokens, large head": (torch.bfloat16, 4, 2, 128, 64, 0, [90, 200], [200, 0], None),
     "many tokens, large head, window": (torch.bfloat16, 6, 2, 96, 32, 45, [150], [100], None),
     "small pages": (torch.bfloat16, 4, 2, 96, 8, 0, [60, 20], [40, 90], None),
