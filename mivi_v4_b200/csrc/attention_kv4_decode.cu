@@ -52,8 +52,10 @@ namespace {
 // blocks (300 rows of one sequence: 5.0 us whole, 6.6 us in two; 1,000 rows behind a window: 10.8 us in pieces of 8, 9.6 us in pieces of 4).
 constexpr int KD_WARPS = 4, KD_KEYS = 64, KD_WHOLE = 8;
 // A weight p * step is at most 2^15 in a column's unit (p up to 2^8, the step below 2 of them times 2^6); steps that lie further apart than
-// 2^KD_SPREAD are not weighed in one unit.
+// 2^KD_SPREAD are not weighed in one unit.  A score beyond KD_FAR less its maximum is worked out by itself: in one step with the product that
+// makes it, the one is rounded and the other is not, and 2^-24 of a score of 2^31 is more than an exponential takes.
 constexpr int KD_ROOM = 6, KD_SPREAD = 8, KD_UNIT_MIN = -120;
+constexpr float KD_FAR = 1048576.0f;
 
 __device__ __forceinline__ void bulk_load(unsigned dst, const void* src, unsigned bytes, unsigned bar) {
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
@@ -461,20 +463,29 @@ attention_kv4_decode_kernel(const __nv_bfloat16* __restrict__ q, const unsigned 
             moves = moves || mx[nt] > m[nt] + 8.f;
         }
         if (__any_sync(0xffffffffu, moves)) {
+            bool far = false;
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
                 for (int d = 4; d < 32; d <<= 1) mx[nt] = fmaxf(mx[nt], __shfl_xor_sync(0xffffffffu, mx[nt], d));
                 mx[nt] = fmaxf(mx[nt], m[nt]);
+                far = far || (fabsf(mx[nt]) > KD_FAR && fabsf(mx[nt]) < INFINITY);
+            }
+            wide = __any_sync(0xffffffffu, wide || far);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
                 const float corr = m[nt] == -INFINITY ? 0.f : ex2(m[nt] - mx[nt]);
                 float of = corr;
                 if (wide) {
                     // the column's own unit: the most that a row which it sees can bring, its weight times its step, is 2^14 of it or less; it never
                     // falls, relative to 1
+                    const float from = mx[nt] == -INFINITY ? 0.f : mx[nt];
                     float my = -INFINITY;
 #pragma unroll
-                    for (int r = 0; r < 8; ++r)
-                        if (sv[r] > 0.f) my = fmaxf(my, __fmul_rn(s[nt][r], lsc[nt]) - mx[nt] + (float)((int)(__float_as_uint(sv[r]) >> 23) - 126));
+                    for (int r = 0; r < 8; ++r) {
+                        s[nt][r] = __fmul_rn(s[nt][r], lsc[nt]) - from;
+                        if (sv[r] > 0.f) my = fmaxf(my, s[nt][r] + (float)((int)(__float_as_uint(sv[r]) >> 23) - 126));
+                    }
 #pragma unroll
                     for (int d = 4; d < 32; d <<= 1) my = fmaxf(my, __shfl_xor_sync(0xffffffffu, my, d));
                     const int unit = 127 - (int)(__float_as_uint(down[nt]) >> 23);
@@ -499,14 +510,15 @@ attention_kv4_decode_kernel(const __nv_bfloat16* __restrict__ q, const unsigned 
             unsigned pe[NT][2], po[NT][2];                       // even columns: the first 16 keys; odd ones: the second 16
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-                const float ref = m[nt] == -INFINITY ? 0.f : -m[nt];        // (0 while a column has seen nothing: its weights come out as 0)
+                // (0 while a column has seen nothing: its weights come out as 0; wide: the scores are relative to it already)
+                const float ref = wide || m[nt] == -INFINITY ? 0.f : -m[nt], to_log2 = wide ? 1.f : lsc[nt];
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
                     float w[2];
 #pragma unroll
                     for (int k = 0; k < 2; ++k) {
                         const int r = 4 * b + 2 * k + j;
-                        const float p = ex2(fmaf(s[nt][r], lsc[nt], ref));  // (ex2(-infinity) is 0: a key that is not seen)
+                        const float p = ex2(fmaf(s[nt][r], to_log2, ref));  // (ex2(-infinity) is 0: a key that is not seen)
                         l[nt] += p;
                         pz[nt] = fmaf(p, zv[r], pz[nt]);
                         w[k] = p * sv[r] * down[nt];

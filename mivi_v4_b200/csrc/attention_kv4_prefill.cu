@@ -58,6 +58,9 @@ static_assert(KQ_OWN % 16 == 0, "read 16 bytes at a time");
 // A row's weights are at most 2^(RESCALE_ABOVE + WEIGHT_ROOM) in its unit, which half precision holds; beside the largest so far they keep their
 // 11 bits down to 2^-21 of it, and what is below 2^-32 of it is lost.
 constexpr float RESCALE_ABOVE = 8.0f, WEIGHT_ROOM = 7.0f;
+// Scores are sums of products below 2^8 times a factor.  Where that is more than FAR a score's difference from its maximum is worked out by itself,
+// as for keys that are uneven: in one step with the factor, the one is rounded and the other is not, and weights pass half's range.
+constexpr float FAR = 16384.0f;
 
 enum { B_Q = 0, B_KFULL = B_Q + TILES, B_KEMPTY = B_KFULL + STAGES, B_VFULL = B_KEMPTY + STAGES, B_VEMPTY = B_VFULL + STAGES,
        B_SFULL = B_VEMPTY + STAGES, B_PFULL = B_SFULL + TILES, B_PVDONE = B_PFULL + TILES, B_SFREE = B_PVDONE + TILES, B_SEGFULL = B_SFREE + TILES, B_SEGEMPTY = B_SEGFULL + 4,
@@ -556,7 +559,7 @@ attention_kv4_prefill_kernel(const __nv_bfloat16* __restrict__ q, const unsigned
             float m = -INFINITY, l = fine ? 0.f : NAN;           // m: the row's reference, log2 units
             float rel = 0.f;                                     // the accumulator's unit is 2^(rel - WEIGHT_ROOM) of what weights relative to 2^m come to
             int j = 0;
-            bool uneven = false;                                 // (the same for all threads)
+            bool uneven = false;
             auto hand_over = [&]() {
                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -626,10 +629,10 @@ attention_kv4_prefill_kernel(const __nv_bfloat16* __restrict__ q, const unsigned
                         const int2 x = e[c];
                         f[c] = scale_log2 * pow2f(max(-126, min(120, ex + x.x)));
                         ev[c] = __int_as_float(x.y);
-                        uneven = uneven || x.y == UNEVEN;
+                        uneven = uneven || x.y == UNEVEN || f[c] > FAR;
                     }
                     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-                    if (uneven) break;
+                    if (__any_sync(0xffffffffu, uneven)) break;
                     free_scores();
                     const int key0 = (sg->kb + j) * BKV;
                     // warp-uniform: some row of the half does not see the whole block
@@ -704,7 +707,7 @@ attention_kv4_prefill_kernel(const __nv_bfloat16* __restrict__ q, const unsigned
                     }
                     hand_over();
                 }
-                if (!ok || !uneven) break;
+                if (!__any_sync(0xffffffffu, ok && uneven)) break;
                 // Every key has powers of two of its own: its score is taken by itself, and its weight and its values' size are added up apart.  (A
                 // path of its own, outside of the loop, which reads the scores from tensor memory again.  400 and 700 tokens behind 6,000 and 12,000, which
                 // never come here, take 163 us so, 214 us where the scores are held in registers through it, and 159 us without it.)

@@ -189,8 +189,10 @@ def test_one_large_value_row(monkeypatch, name, where, power):
     hold_to_weights(out, q, ks, vs, lens, before, window, dtype, page, teeth=0.5)
 
 
-@pytest.mark.parametrize("power", [12, 20])
-@pytest.mark.parametrize("name", SHAPES)
+# (2^60: scores that 32 bits round by more than an exponential takes.  The kernels that rows read back in bfloat16 go to, those of a bfloat16
+# cache, are not made for them.)
+@pytest.mark.parametrize("name,power", [(n, p) for n, x in SHAPES.items() for p in (12, 20, 40, 60)
+                                        if not (p > 20 and x[0] == torch.bfloat16 and n.startswith("small pages, read back"))])
 def test_one_large_key_row(monkeypatch, name, power):
     """One key row 2^power times as large as the others: the last token's, or one behind a window, whose value is small; and one that every query sees far
     below the best."""
