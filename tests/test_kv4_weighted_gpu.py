@@ -66,11 +66,11 @@ def weighed(q, k, v, first, window, dtype, form):
     return want, room, (((mean - want).abs() > room) & (want.abs() > room)).flatten(1).any(-1)
 
 
-def hold_to_weights(out, q, ks, vs, lens, before, window, dtype, page, teeth=0.9):
-    """Every row of the step against the formula; ks, vs: what the sequences' rows stand for."""
+def hold_to_weights(out, q, ks, vs, lens, before, window, dtype, page, teeth=0.9, forms=None):
+    """Every row of the step against the formula; ks, vs: what the sequences' rows stand for; forms: a sequence's kernel where it is not the usual one."""
     n = telling = 0
     for b, (m, first) in enumerate(zip(lens, before)):
-        form = kernel_of(dtype, q.shape[-1], page, lens, m)
+        form = forms or kernel_of(dtype, q.shape[-1], page, lens, m)
         want, room, tells = weighed(q[n:n + m], ks[b], vs[b], first, window, dtype, form)
         got = out[n:n + m].double().cpu()
         assert torch.isfinite(got).all(), (b, form)
@@ -247,3 +247,44 @@ def test_values_of_every_size(monkeypatch, name):
             ys.append((k, v))
         out, ks, vs = run(shape, q, ys)
         hold_to_weights(out, q, ks, vs, lens, before, window, dtype, page, teeth=0.5)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("nh,nkv,hd,page,window", [(32, 8, 64, 64, 0), (3, 1, 64, 64, 0), (6, 2, 128, 16, 0), (5, 5, 48, 32, 50), (8, 2, 64, 64, 70),
+                                                   (4, 2, 40, 8, 0), (2, 1, 256, 64, 0), (16, 8, 96, 64, 0), (4, 2, 96, 8, 0), (3, 1, 80, 1, 60), (2, 1, 256, 8, 0)])
+@pytest.mark.parametrize("lens", [[17, 1, 300], [260, 140], [3, 64, 16, 17, 1]])
+def test_runs_of_all_lengths(dtype, nh, nkv, hd, page, window, lens):
+    """More than 16 tokens, and steps with both, of every head size, type and page size: over the codes, on tcgen05 and read back."""
+    before = [0, 200, 63, 64, 1][:len(lens)]
+    shape = (dtype, nh, nkv, hd, page, window, lens, before, None)
+    g = torch.Generator().manual_seed(nh + sum(lens))
+    xs = []
+    for m, c in zip(lens, before):                               # keys with a channel that stands out, values whose size changes from row to row
+        k, v = torch.randn(2, m + c, nkv, hd, generator=g)
+        k[..., 0] *= 4
+        xs.append((k, v * torch.exp(torch.randn(m + c, nkv, 1, generator=g))))
+    q = torch.randn(sum(lens), nh, hd, generator=g).to(dtype)
+    out, ks, vs = run(shape, q, xs)
+    hold_to_weights(out, q, ks, vs, lens, before, window, dtype, page)
+
+
+def test_more_rows_than_the_tables_of_the_many_token_kernel_hold(monkeypatch):
+    """Such a step goes over the codes."""
+    monkeypatch.setattr(K(), "KV4_PREFILL_MOST", 4)
+    monkeypatch.setattr(K(), "_attention_kv4_prefill", None)
+    shape = (torch.bfloat16, 8, 1, 64, 64, 0, [130], [0], None)
+    q, xs, _ = queries_and_rows(shape, 8)
+    out, ks, vs = run(shape, q, xs)
+    hold_to_weights(out, q, ks, vs, [130], [0], 0, torch.bfloat16, 64, forms="codes")
+
+
+def test_the_bound_has_teeth():
+    """Zeros, and the mean of what is seen, are out of it by far; a result that is right to its last place is within it."""
+    for dtype, hd, form in ((torch.bfloat16, 128, "codes"), (torch.bfloat16, 64, "half"), (torch.bfloat16, 96, "back"), (torch.float32, 64, "core"),
+                            (torch.float32, 96, "back")):
+        shape = (dtype, 4, 2, hd, 64, 0, [40], [460], None)
+        q, xs, _ = queries_and_rows(shape, 9)
+        _, _, (k,), (v,) = in_pages(xs, 64, 1)
+        want, room, tells = weighed(q, k, v, 460, 0, dtype, form)
+        assert tells.all() and ((want.to(dtype).double() - want).abs() <= room).all()
+        assert float(room.max()) < (0.5 if form == "back" else 0.1) * float(want.abs().max())
