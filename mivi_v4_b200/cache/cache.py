@@ -114,10 +114,11 @@ def rows_of_4_bits(pages: torch.Tensor, page_size: int, head_dim: int) -> torch.
     """What pages held in 4 bits stand for: uint8 [..., kv heads, page_size * (head_dim + 8)] -> float32
     [..., 2, kv heads, page_size, head_dim].  For inspection, on any device; steps read rows back with kernels."""
     codes = pages[..., :page_size * head_dim].unflatten(-1, (2, page_size, head_dim // 2))
-    codes = torch.stack([codes & 15, codes >> 4], dim=-1).flatten(-2).float()
-    params = pages[..., page_size * head_dim:].contiguous().view(torch.bfloat16).unflatten(-1, (page_size, 2, 2)).float()
+    codes = torch.stack([codes & 15, codes >> 4], dim=-1).flatten(-2).double()
+    params = pages[..., page_size * head_dim:].contiguous().view(torch.bfloat16).unflatten(-1, (page_size, 2, 2)).double()
     params = params.transpose(-3, -2)                      # [..., kv heads, K or V, row, (step, zero)]
-    return (params[..., 1:2] + codes * params[..., 0:1]).movedim(-3, -4)
+    # (in 64 bits: 15 steps may pass the largest float32 where a row's ends do not)
+    return (params[..., 1:2] + codes * params[..., 0:1]).float().movedim(-3, -4)
 
 
 class _Slot:
