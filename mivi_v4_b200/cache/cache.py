@@ -16,7 +16,8 @@ state per layer in its run state (crates/mivi-core/src/arena.rs:56,82,105);
 both have one sequence.  Slots, pages and groups are this library's own.
 
 All bookkeeping is on the host; only the storage lives on the device.  Nothing
-here launches a kernel except zeroing a slot's state.  Beside the page lists of
+here launches a kernel except zeroing a slot's state and looking at rows that are
+held in 4 bits (``dump_slot``).  Beside the page lists of
 each sequence the cache keeps the same facts as arrays over all slots (lengths,
 page tables), so that a decode step of many sequences reads and advances them
 without a loop over the sequences.
@@ -112,7 +113,8 @@ class StateView:
 
 def rows_of_4_bits(pages: torch.Tensor, page_size: int, head_dim: int) -> torch.Tensor:
     """What pages held in 4 bits stand for: uint8 [..., kv heads, page_size * (head_dim + 8)] -> float32
-    [..., 2, kv heads, page_size, head_dim].  For inspection, on any device; steps read rows back with kernels."""
+    [..., 2, kv heads, page_size, head_dim].  In torch operations, on any device; a cache on a GPU reads rows back with
+    ``ops.kernels.kv4_read``, to the same values."""
     codes = pages[..., :page_size * head_dim].unflatten(-1, (2, page_size, head_dim // 2))
     codes = torch.stack([codes & 15, codes >> 4], dim=-1).flatten(-2).double()
     params = pages[..., page_size * head_dim:].contiguous().view(torch.bfloat16).unflatten(-1, (page_size, 2, 2)).double()
@@ -371,6 +373,8 @@ class SequenceCache:
                     else:
                         vs[:, lo:hi] = st[:, page, nkv * ps * dk:].view(-1, nkv, ps, dv)[:, :, :hi - lo].permute(0, 2, 1, 3)
                 out[gi] = (ks, vs)
+            elif isinstance(g.need, KVNeed) and g.need.bits and st.is_cuda:
+                out[gi] = self._read_4_bits(gi, slot)
             elif isinstance(g.need, KVNeed):
                 L = int(self._len[slot])
                 rows = torch.zeros((g.n_layers, 2, L, g.need.n_kv_heads, g.need.head_dim),
@@ -385,6 +389,25 @@ class SequenceCache:
             else:
                 out[gi] = st[:, slot].clone()
         return out
+
+    def _read_4_bits(self, gi: int, slot: int) -> torch.Tensor:
+        """The rows of ``slot`` in a group held in 4 bits, on its GPU: float32 [layers, 2, length, kv heads, head_dim]."""
+        from ..ops import kernels as K
+        g, st, L, ps = self.plan.groups[gi], self.storage[gi], int(self._len[slot]), self.page_size
+        nkv, hd = g.need.n_kv_heads, g.need.head_dim
+        pages = self._get(slot).pages[gi]
+        rows = torch.zeros((g.n_layers, 2, L, nkv, hd), dtype=torch.float32, device=st.device)
+        kept = [t for blk, page in enumerate(pages) if page is not None for t in range(blk * ps, min(L, (blk + 1) * ps))]
+        if not kept:
+            return rows
+        with torch.cuda.device(st.device):
+            positions = torch.tensor(kept, dtype=torch.int32, device=st.device)
+            table = torch.tensor(self.page_rows(gi, [slot]), dtype=torch.int32, device=st.device)
+            got = torch.empty((2, len(kept), nkv, hd), dtype=torch.float32, device=st.device)
+            for layer in range(g.n_layers):
+                K.kv4_read(st[layer], table, positions, torch.zeros_like(positions), got[0], got[1], nkv, hd)
+                rows[layer, :, kept] = got
+        return rows
 
     def check(self) -> None:
         """No slot or page lost, held twice or freed twice."""
