@@ -874,8 +874,9 @@ attention_kv4_prefill_kernel(const __nv_bfloat16* __restrict__ q, const unsigned
 }  // namespace
 
 // bfloat16, heads of 8 to 64 in steps of 8.  cu and starts are those of ``n_seqs`` neighbouring sequences (cu counts from q's first row), page_table their rows; at most
-// 1,024 sequences of at least one token, and 1,024 tiles of 256 rows (a sequence's tokens times the heads of a kv head).  whole: a block a tile and
-// kv head (grid: tiles * nkv); else grid blocks, one a multiprocessor at most, share all key blocks.  part_o [2 grid, 16, 256, 4],
+// 1,024 sequences of at least one token, and 1,024 tiles of 256 rows (a sequence's tokens times the heads of a kv head).  whole: tiles and
+// kv heads are dealt out whole to grid blocks (tiles * nkv at most), back and forth; else grid blocks share all key blocks.  Either way a block a
+// multiprocessor at most.  part_o [2 grid, 16, 256, 4],
 // part_ml [2 grid, 256, 2] float32 and tickets [tiles * nkv] (zero) are used unless whole.
 MV_API int mv_attention_kv4_prefill(const void* q, const void* pool, const int* page_table, int table_stride, int page_size, const int* cu,
                                     const int* starts, void* o, float* part_o, float* part_ml, int* tickets, int n_seqs, int nh, int nkv, int hd,

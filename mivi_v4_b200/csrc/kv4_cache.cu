@@ -669,16 +669,11 @@ MV_API int mv_attention_kv4(const void* record) {
     int page_shift = 0;
     while ((1 << page_shift) < page_size) ++page_shift;
     const dim3 grid(splits, nkv * head_tiles, N);
-    cudaError_t attr = cudaSuccess;
+    // (at most 4 * (5 * 4 * 256 + 8 * 4) bytes: less than any block may have)
 #define MV_GO(T, GT)                                                                                                              \
-    do {                                                                                                                          \
-        const size_t smem = sizeof(float) * (5 * GT * hd + 8 * GT);                                                               \
-        if (smem > 48 * 1024) attr = mv_allow_smem<attention_kv4_kernel<T, GT>>(sizeof(float) * (5 * GT * KV4_MAX_HEAD_DIM + 8 * GT)); \
-        if (attr != cudaSuccess) return (int)attr;                                                                                \
-        mv_launch(attention_kv4_kernel<T, GT>, grid, 128, smem, stream, (const T*)q, (const unsigned char*)pool, page_table,       \
-                  table_stride, page_shift, positions, seq_of, (T*)o, part_o, part_ml, tickets, nh, nkv, hd, scale, window,        \
-                  head_tiles);                                                                                                    \
-    } while (0)
+    mv_launch(attention_kv4_kernel<T, GT>, grid, 128, sizeof(float) * (5 * GT * hd + 8 * GT), stream, (const T*)q,                 \
+              (const unsigned char*)pool, page_table, table_stride, page_shift, positions, seq_of, (T*)o, part_o, part_ml, tickets, \
+              nh, nkv, hd, scale, window, head_tiles)
 #define MV_GT(T)                                                                                                                  \
     do {                                                                                                                          \
         if (gt == 1) MV_GO(T, 1);                                                                                                 \

@@ -2933,8 +2933,8 @@ def _attention_kv4_direct(q, pool, page_table, W, page_size, positions, seq_of, 
         return
     gt, head_tiles, auto = attention_kv4_plan(N, nh, nkv, W * page_size)
     splits = auto if splits is None else int(splits)
-    if N > 65535 or nkv * head_tiles > 65535:
-        raise KernelError(f"attention_kv4: {N} tokens and {nkv} kv heads in one launch; each may be 65535 at most")
+    if nkv * head_tiles > 65535:
+        raise KernelError(f"attention_kv4: {nh} heads of {nkv} kv heads make {nkv * head_tiles} tiles, 65535 at most in a launch")
     part_o = part_ml = tickets = 0
     if splits > 1:
         part_o = ws.get("attn_part_o", (N * nh * splits * hd,), torch.float32).data_ptr()
