@@ -2795,9 +2795,9 @@ def attention_kv4(q: torch.Tensor, pool: torch.Tensor, page_table, positions, se
         raise KernelError(f"attention: {nh} heads are not a multiple of {nkv} kv heads")
     if out.dtype != q.dtype:
         raise KernelError(f"attention: q {q.dtype} and out {out.dtype} must agree")
-    if len(host_starts) != B or sum(host_lens) != N or (B and min(host_lens) < 1):
+    if len(host_starts) != B or sum(host_lens) != N or (B and (min(host_lens) < 1 or min(host_starts) < 0)):
         raise KernelError(f"attention_kv4: {len(host_starts)} starts and {B} lengths of {sum(host_lens)} tokens for {N} rows of q; every "
-                          "sequence brings a token or more")
+                          "sequence brings a token or more, from position 0 or later on")
     if not 0.0 < scale < 1e4:
         raise KernelError(f"attention_kv4: scale {scale}, expected a positive number")
     if splits is not None and not 1 <= int(splits) <= 1024:
