@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import operator
 import os
 import struct
 from dataclasses import dataclass
@@ -2826,7 +2827,7 @@ def attention_kv4(q: torch.Tensor, pool: torch.Tensor, page_table, positions, se
     max_len, reach = max(host_lens), max(host_starts)
     reach += max_len
     if reach > W * page_size:
-        reach = max(map(int.__add__, host_starts, host_lens))
+        reach = max(map(operator.add, host_starts, host_lens))       # (numbers of numpy too)
         if reach > W * page_size:
             raise KernelError(f"attention_kv4: {reach} tokens in a sequence, the page table reaches {W * page_size}")
     if max_len <= KV4_DIRECT_TOKENS:
