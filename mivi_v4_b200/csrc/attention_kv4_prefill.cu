@@ -49,7 +49,9 @@ constexpr int Q_BYTES = BQ * HD * 2, KV_BYTES = BKV * HD * 2, P_BYTES = BQ * BKV
 constexpr int STAGES = 3, EXPS = 8, KQ_MOST = 1024;              // most sequences, and most tiles, of a launch
 constexpr int KQ_EXTRA = 3;                                      // key blocks that a tile's beginning and end count for
 constexpr int UNEVEN = 0x7f800000;
-constexpr int KQ_SPREAD = 8;                                     // rows of 32 whose sizes are within this many powers of two share theirs
+// Rows of 32 whose sizes are within KQ_SPREAD powers of two share theirs: the largest's comes to 2^KQ_LIFT, so that a row 2^-12 of it is still 2^15 times the
+// least normal half, and whichever row has the weight, its weight is within 2^12 of the largest there can be.
+constexpr int KQ_SPREAD = 12, KQ_LIFT = 13;
 constexpr int KQ_BARS = TILES * Q_BYTES + 2 * STAGES * KV_BYTES + TILES * P_BYTES, KQ_EXPS = KQ_BARS + 272, KQ_SEGS = KQ_EXPS + EXPS * 32, KQ_TABLES = KQ_SEGS + 4 * 96,
               KQ_OWN = KQ_TABLES + (3 * KQ_MOST + 4) * 4, KQ_SMEM = KQ_OWN + EXPS * BKV * 4 + 1024;
 static_assert(KQ_SMEM <= 227 * 1024 - 512, "shared memory");
@@ -58,9 +60,9 @@ static_assert(KQ_OWN % 16 == 0, "read 16 bytes at a time");
 // A row's weights are at most 2^(RESCALE_ABOVE + WEIGHT_ROOM) in its unit, which half precision holds; beside the largest so far they keep their
 // 11 bits down to 2^-21 of it, and what is below 2^-32 of it is lost.
 constexpr float RESCALE_ABOVE = 8.0f, WEIGHT_ROOM = 7.0f;
-// Scores are sums of products below 2^8 times a factor.  Where that is more than FAR a score's difference from its maximum is worked out by itself,
+// Scores are sums of products below 2^(8 + KQ_LIFT) times a factor.  Where that is more than FAR a score's difference from its maximum is worked out by itself,
 // as for keys that are uneven: in one step with the factor, the one is rounded and the other is not, and weights pass half's range.
-constexpr float FAR = 16384.0f;
+constexpr float FAR = 2.0f;
 
 enum { B_Q = 0, B_KFULL = B_Q + TILES, B_KEMPTY = B_KFULL + STAGES, B_VFULL = B_KEMPTY + STAGES, B_VEMPTY = B_VFULL + STAGES,
        B_SFULL = B_VEMPTY + STAGES, B_PFULL = B_SFULL + TILES, B_PVDONE = B_PFULL + TILES, B_SFREE = B_PVDONE + TILES, B_SEGFULL = B_SFREE + TILES, B_SEGEMPTY = B_SEGFULL + 4,
@@ -81,6 +83,8 @@ __device__ __forceinline__ unsigned long long smem_desc_mn(unsigned addr) {
 __device__ __forceinline__ unsigned instr_desc_half(int m, int n) { return (1u << 4) | ((unsigned)(n >> 3) << 17) | ((unsigned)(m >> 4) << 24); }
 __device__ __forceinline__ float pow2f(int e) { return __uint_as_float((unsigned)(e + 127) << 23); }       // e from -126 to 127
 __device__ __forceinline__ int exponent(unsigned bits) { return max(-126, min(126, (int)(bits >> 23) - 127)); }
+// the unit of a row's halves: 2^-KQ_LIFT of its largest element's power of two
+__device__ __forceinline__ int unit_of(unsigned bits) { return max(-126, (int)(bits >> 23) - 127 - KQ_LIFT); }
 
 // The 8 codes of a word as four pairs of halves, each step * code + zero (rounded once)
 __device__ __forceinline__ uint4 elements(unsigned w, unsigned step, unsigned zero) {
@@ -375,12 +379,12 @@ attention_kv4_prefill_kernel(const __nv_bfloat16* __restrict__ q, const unsigned
                 const float big_k = fmaxf(fabsf(p.kz), fabsf(fmaf(15.f, p.ks, p.kz))), big_v = fmaxf(fabsf(p.vz), fabsf(fmaf(15.f, p.vs, p.vz)));
                 const unsigned bits_k = big_k < INFINITY ? __float_as_uint(big_k) : 0u, bits_v = __float_as_uint(big_v);
                 const unsigned top_k = __reduce_max_sync(0xffffffffu, bits_k), top_v = __reduce_max_sync(0xffffffffu, bits_v);
-                int ek = exponent(top_k), ev = exponent(top_v);
+                int ek = unit_of(top_k), ev = unit_of(top_v);
                 // (a key of zeros scores 0 in any unit; a value of zeros may have the weight that the others' are to be measured by)
                 const bool uneven = __any_sync(0xffffffffu, there && ((bits_k != 0u && bits_k + (KQ_SPREAD << 23) < top_k) || bits_v + (KQ_SPREAD << 23) < top_v));
                 if (uneven) {
-                    ek = exponent(bits_k);
-                    ev = exponent(bits_v);
+                    ek = unit_of(bits_k);
+                    ev = unit_of(bits_v);
                 }
                 auto put = [&](unsigned char* stage, const uint4 (&w)[2], float step, float zero, float down) {
                     const unsigned st = twice(step * down), z = twice(zero * down);
@@ -710,7 +714,8 @@ attention_kv4_prefill_kernel(const __nv_bfloat16* __restrict__ q, const unsigned
                 if (!__any_sync(0xffffffffu, ok && uneven)) break;
                 // Every key has powers of two of its own: its score is taken by itself, and its weight and its values' size are added up apart.  (A
                 // path of its own, outside of the loop, which reads the scores from tensor memory again.  400 and 700 tokens behind 6,000 and 12,000, which
-                // never come here, take 163 us so, 214 us where the scores are held in registers through it, and 159 us without it.)
+                // never come here, take 163 us so, 214 us where the scores are held in registers through it, and 161 us without it.  A block that
+                // comes here takes some four times as long.)
                 const int past = pos - (sg->kb + j) * BKV + 1, from = window > 0 ? past - window : 0;
                 auto each = [&](auto use) {                      // use(32 keys, i, score in log2 units, its values' power of two)
 #pragma unroll 1

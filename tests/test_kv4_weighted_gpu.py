@@ -24,10 +24,10 @@ def weighed(q, k, v, first, window, dtype, form):
     """(wanted, how far off a result may be, whether the mean of what is seen is out of that) of the queries [m, nh, hd] at positions first, first + 1, ...
 
     A score of query q and key k may be off by scale times: the query's rounding (codes: whole numbers of 16 bits whose largest is 2^14 or more, so
-    2^-15 of the largest element an element; half, back: none to speak of), the key's (half: 2^-11 of an element and, below half's normal numbers, 2^-13 of the
-    row's largest, rows of 2^8 times its size sharing its power of two; query elements 2^-11; back in bfloat16: 2^-8), and sums in 32 bits, hd
+    2^-15 of the largest element an element; half, back: none to speak of), the key's (half: 2^-11 of an element and, below half's normal numbers, 15 * 2^-25 for a
+    row whose largest is 2 or more, rows of 2^12 times its size sharing its power of two: 2^-22 of it; query elements 2^-11; back in bfloat16: 2^-8), and sums in 32 bits, hd
     steps of 2^-24 of sum |q| (|zero| + 15 step), taken as twice sum |q| max |k|.  A score off by e makes its weight off by exp(e) - 1.  Weights are rounded
-    by 2^-11 (codes, half) or 2^-8 (back in bfloat16), values by 2^-11 + 2^-13 of the row's largest (half) or 2^-8 (back); sums of T weighted
+    by 2^-11 (codes, half) or 2^-8 (back in bfloat16), values by 2^-11 + 2^-22 of the row's largest (half) or 2^-8 (back); sums of T weighted
     values and T weights in 32 bits, 4 sqrt(T) 2^-24, the exponential's last places 2^-20.  The result's own rounding is 2^-8 or 2^-24 of it, and below
     bfloat16's or float32's normal numbers nothing is asked for."""
     m, nh, hd = q.shape
@@ -49,7 +49,7 @@ def weighed(q, k, v, first, window, dtype, form):
         if form == "codes":
             e = e + 2.0 ** -15 * q_top * kk.abs().sum(-1)
         if form == "half":
-            e = e + 2 * 2.0 ** -11 * mags + 2.0 ** -13 * q_sum * k_top
+            e = e + 2 * 2.0 ** -11 * mags + 2.0 ** -22 * q_sum * k_top
         if form == "back" and bf:
             e = e + 2.0 ** -8 * mags
         off = ((logp + e * scale).exp() - p).clamp_max(1.0) + 2.0 ** -20 * p
@@ -58,7 +58,7 @@ def weighed(q, k, v, first, window, dtype, form):
         lost = off.sum(-1, keepdim=True)
         open_ = lost > 0.5                                       # (scores too large to be told apart: only a mean of what is seen is asked for)
         lost = lost.clamp_max(0.5)
-        weight = {"core": 0.0, "codes": 2.0 ** -11, "half": 2 * 2.0 ** -11 + 2.0 ** -13, "back": 2 * 2.0 ** -8 if bf else 0.0}[form] + 4 * T ** 0.5 * 2.0 ** -24
+        weight = {"core": 0.0, "codes": 2.0 ** -11, "half": 2 * 2.0 ** -11 + 2.0 ** -22, "back": 2 * 2.0 ** -8 if bf else 0.0}[form] + 4 * T ** 0.5 * 2.0 ** -24
         room[:, h] = (off @ vv.abs() + lost * want[:, h].abs()) / (1 - lost) + weight * (p @ v_top)[:, None]
         room[:, h] += open_ * 2 * (seen * v_top).amax(-1, keepdim=True)
         mean[:, h] = (seen @ vv) / seen.sum(-1, keepdim=True)
