@@ -13,7 +13,7 @@
 // or 16 of them, so what is lost is 2^-16 of that; a bfloat16 element within 2^-7 of it is exact), in two pieces of 8 bits that take
 // neighbouring columns: the 4 heads that usually share a kv head fill the 8 columns, and a lane's two accumulators are one score's two
 // pieces.  (In half precision a pair of codes costs 1.2 instructions each, twice the products, and half of the columns stay empty: 746
-// instructions a tile of 64 keys against some 590 now, both with what a piece costs besides its tiles.)
+// instructions a tile of 64 keys against some 620 now, both with what a piece costs besides its tiles.)
 //
 // Weights times values: m16n8k16 in half precision, whose 11 bits a weight needs (whole numbers of 15 bits lose those that lie far below the
 // largest).  Codes less 8 are exact in it and cost 1.25 instructions a code: merge two keys' words, mask a nibble of each into the mantissas
@@ -35,9 +35,9 @@
 // that the device is filled.  So unequal sequences are balanced, and a recorded launch fits any lengths it is replayed with.  Warps merge
 // in shared memory, pieces in order by the block that finishes last (ticket counter, left at 0).
 //
-// Measured, 32 / 8 heads of 64: 8 sequences of 32,768 rows, 151 MB, 37.1 us, 4.07 TB/s or 0.62 of a copy's rate: instructions are issued in 0.55
+// Measured, 32 / 8 heads of 64: 8 sequences of 32,768 rows, 151 MB, 37.9 us, 3.98 TB/s or 0.61 of a copy's rate: instructions are issued in 0.56
 // of the clocks, by 14 warps a multiprocessor, which wait for one another's results (fixed latencies) and for loads in equal parts.
-// 8 sequences of 512 to 4,096: 9.9 us; one of 301, where there is next to nothing to read: 4.7 us.  (The same 8 of 32,768 in bfloat16, 537 MB,
+// 8 sequences of 512 to 4,096: 10.0 us; one of 301, where there is next to nothing to read: 4.9 us.  (Where steps lie far apart: 43 us for the 32,768.)  (The same 8 of 32,768 in bfloat16, 537 MB,
 // take attention_decode_tc.cu 87 us.)
 #include "kv4.cuh"
 #include "tc_common.cuh"
@@ -75,7 +75,8 @@ __device__ __forceinline__ unsigned transpose8x8(unsigned a) {
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
     return d;
 }
-// nibbles 0 and 1 of both halves of x as pairs of halves, less 8: 1024 + c - 1032, and (1024 + 16 c) / 16 - 72
+// nibbles 0 and 1 of both halves of x as pairs of halves, less 8: 1024 + c - 1032, and (1024 + 16 c) / 16 - 72 (whole numbers put into the mantissa of a
+// known power of two: Kim, Henry, Fahim and Awadalla, "Who Says Elephants Can't Run", 2022)
 __device__ __forceinline__ void centred(unsigned x, unsigned& even, unsigned& odd) {
     unsigned e, o;
     asm("lop3.b32 %0, %1, 0x000f000f, 0x64006400, 0xea;" : "=r"(e) : "r"(x));

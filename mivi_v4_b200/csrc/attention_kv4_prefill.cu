@@ -15,8 +15,8 @@
 // One block a multiprocessor at most, and two ways to share the work out (``attention_kv4_prefill_plan`` takes the quicker): whole tiles and kv
 // heads, the longest first, where there are enough of them; or to each block the same share of all tiles' and kv heads' key blocks
 // (128 keys of a tile, and some for a tile's beginning and end), where a block begins and ends in the middle of a tile's keys and the block
-// that finishes a tile last puts its parts together.  2,048 tokens of a prompt, 32 / 8 heads: 50 us whole, 62 us in shares; 700 and 400 tokens
-// behind 6,000 and 12,000: 202 us whole (the longest tiles alone), 161 us in shares.
+// that finishes a tile last puts its parts together.  2,048 tokens of a prompt, 32 / 8 heads: 49 us whole, 66 us in shares; 700 and 400 tokens
+// behind 6,000 and 12,000: 210 us whole (the longest tiles alone), 163 us in shares.
 //
 //   warps 0 - 3    operands, a key a thread: codes and numbers of a key block, a block ahead in registers, into rings of three stages each in the
 //                  128-byte swizzle.  A word's eight codes come out as pairs (0, 4), (1, 5), (2, 6), (3, 7) by masking them into the mantissa of
@@ -86,7 +86,8 @@ __device__ __forceinline__ int exponent(unsigned bits) { return max(-126, min(12
 // the unit of a row's halves: 2^-KQ_LIFT of its largest element's power of two
 __device__ __forceinline__ int unit_of(unsigned bits) { return max(-126, (int)(bits >> 23) - 127 - KQ_LIFT); }
 
-// The 8 codes of a word as four pairs of halves, each step * code + zero (rounded once)
+// The 8 codes of a word as four pairs of halves, each step * code + zero (rounded once); the codes by way of the mantissa, as in
+// attention_kv4_decode.cu
 __device__ __forceinline__ uint4 elements(unsigned w, unsigned step, unsigned zero) {
     unsigned e[4];
 #pragma unroll

@@ -2758,7 +2758,7 @@ def kv4_read(pool: torch.Tensor, page_table, positions, seq_of, k_out: torch.Ten
 
 
 # Tokens a sequence up to which a step's queries read the codes themselves, in a kernel made for few.  Heads of 64, 32 / 8 of them: 16 sequences
-# of 6 tokens behind 3,000 take 29 us there and 51 us in the tcgen05 kernel, 8 of 9 behind 2,000 22 and 31, 8 of 20 39 and 31.
+# of 6 tokens behind 3,000 take 30 us there and 52 us in the tcgen05 kernel, 8 of 9 behind 2,000 22 and 34, 8 of 20 39 and 34.
 KV4_DIRECT_TOKENS = 16
 # The same where more tokens have their cache read back (float32, and pages of fewer than 16 tokens): 32 / 8 heads of 64 in float32, 64 tokens behind
 # 2,000 take 124 us over the codes and 393 us read back, 512 of a prompt 147 and 97 us, 1,500 1,120 and 480 us; 3 / 1 heads of 96 280 and 337 us.
@@ -2787,7 +2787,8 @@ def attention_kv4(q: torch.Tensor, pool: torch.Tensor, page_table, positions, se
                   hd: int, scale: float, window: int, ws, host_starts, host_lens, splits: Optional[int] = None) -> torch.Tensor:
     """Causal attention of every token of the step over its sequence's cache held in 4 bits (which already holds the step's own
     keys), optional sliding window: q and out [N, heads * head size] in bfloat16 or float32.  The step's tokens are packed sequence
-    by sequence (``cu``), sequence b bringing ``host_lens[b]`` tokens from position ``host_starts[b]`` = ``starts[b]`` on.  ``ws`` (a
+    by sequence (``cu``), sequence b bringing ``host_lens[b]`` tokens from position ``host_starts[b]`` = ``starts[b]`` on; row b of the page
+    table is its, and names a page of the pool for each of its pages, those behind the window too (any page will do there).  ``ws`` (a
     Workspace) supplies the scratch; ``splits``: into how many parts the longest sequence's keys are cut where the codes are read
     (None: as fills the device)."""
     N, B = q.shape[0], len(host_lens)
@@ -2837,8 +2838,8 @@ def attention_kv4(q: torch.Tensor, pool: torch.Tensor, page_table, positions, se
     args = (pool, page_table, W, page_size, positions, seq_of, starts, out, nh, nkv, hd, scale, window, ws)
     fused = attention_kv4_prefill_supported(dtype, hd) and max_len * (nh // nkv) <= 256 * KV4_PREFILL_MOST
     # Larger heads in bfloat16 stay with the codes, too: rows read back would be off by as much again as the result's own rounding, and take the
-    # memory that 4 bits save.  2,048 tokens of a prompt, 16 / 4 heads of 128: 186 us so, 127 us read back; 64 tokens behind 8,000: 51 and 240.
-    # And so do head sizes that no kernel of many tokens takes in tiles: 8 / 2 heads of 256, 2,048 tokens: 296 us so, 3,840 us read back.
+    # memory that 4 bits save.  2,048 tokens of a prompt, 16 / 4 heads of 128: 196 us so, 128 us read back; 64 tokens behind 8,000: 40 and 240.
+    # And so do head sizes that no kernel of many tokens takes in tiles: 8 / 2 heads of 256, 2,048 tokens: 302 us so, 3,840 us read back.
     few = KV4_DIRECT_TOKENS if fused else KV4_DIRECT_INSTEAD
     if not fused and (max_len <= few or hd > 128 or attention_kv4_decode_supported(dtype, page_size)):
         _attention_kv4_direct(q, *args, cu, 0, N, B, max_len, reach, splits, dt, dev)
@@ -2885,8 +2886,8 @@ def attention_kv4_decode_plan(N: int, nh: int, nkv: int, hd: int, max_len: int):
     operands, and cost registers.  The kernel cuts the keys into equal pieces by the lengths that it finds."""
     G = nh // nkv
     # (few columns in all: narrow tiles, which more blocks take and whose parts are put together sooner.  16 / 1 heads of 64, one token: 1, 4 and 8
-    # sequences of 8,000 take 10.5, 12.4 and 12.9 us so, 16.2, 17.8 and 18.6 us in tiles of 16 columns; 32 of them 24.6 and 18.8 us.  Between,
-    # 16 tokens of one sequence, 32 / 8 heads: behind 300 5.8, 6.7 and 8.8 us in tiles of 4, 8 and 16, behind 8,000 24.3, 19.0 and 19.4 us.)
+    # sequences of 8,000 take 10.8, 12.4 and 12.8 us so, 16.4, 18.0 and 18.7 us in tiles of 16 columns; 32 of them 24.5 and 19.2 us.  Between,
+    # 16 tokens of one sequence, 32 / 8 heads: behind 300 5.7, 6.6 and 9.4 us in tiles of 4, 8 and 16, behind 8,000 24.6, 18.9 and 19.6 us.)
     nt_max = 1 if N * nh <= 256 else 2 if N * nh <= 512 or hd > 128 else 4
     head_tiles = -(-G // (4 * nt_max))
     heads = -(-G // head_tiles)
