@@ -20,7 +20,7 @@
 // of 1024 or 64, subtract.  Half's range is small, so the weights p * step are taken relative to a power of two: the largest step's so far,
 // while no step is below 2^-KD_SPREAD of it.  Where steps lie further apart, the largest step may be a row's that a column does not see or gives no
 // weight, beside which the rows that it does weigh would vanish; there each column has a unit of its own, which follows the most that one of
-// its rows brings (score and step together).
+// its rows brings (score and step together).  (p itself is a 32-bit number: below 2^-126 of the best key's it is 0, whatever it would multiply.)
 //
 // The scores are computed transposed, S^T = K Q^T, keys on a product's 16 rows.  Sums over a row run over elements in any order, so a lane
 // takes the row's bytes as they lie (lane t of four: a quarter of it) and reads its queries to match.  O^T = V^T P^T: a lane takes 8
